@@ -170,6 +170,43 @@ class ReadoutCE(C.Structure):
     ]
 
 
+class Rope(C.Structure):  # hma_rope_t
+    _fields_ = [
+        ("freqs", c_vp), ("axes", c_vp), ("positions", c_vp), ("pos_stride", c_i64),
+        ("q_w", c_vp), ("q_b", c_vp), ("k_w", c_vp), ("k_b", c_vp),
+        ("d", c_i32), ("rot", c_i32), ("interleaved", c_i32), ("norm", c_i32), ("dtype", c_i32), ("w_f32", c_i32), ("pos_64", c_i32),
+        ("n_axes", c_i32),
+        ("eps", c_f32), ("amplitude", c_f32),
+    ]
+
+
+class QkRope(C.Structure):
+    _fields_ = [
+        ("r", Rope),
+        ("tokens", c_i64), ("hq", c_i32), ("hk", c_i32),
+        ("q", c_vp), ("k", c_vp), ("q_tok", c_i64), ("q_head", c_i64), ("k_tok", c_i64), ("k_head", c_i64),
+        ("q_out", c_vp), ("k_out", c_vp),
+        ("dy_q", c_vp), ("dy_k", c_vp), ("dyq_tok", c_i64), ("dyq_head", c_i64), ("dyk_tok", c_i64), ("dyk_head", c_i64),
+        ("dq", c_vp), ("dk", c_vp), ("dq_w", c_vp), ("dq_b", c_vp), ("dk_w", c_vp), ("dk_b", c_vp),
+        ("ws", c_vp), ("ws_floats", c_i64),
+    ]
+
+
+class KvAppend(C.Structure):
+    _fields_ = [
+        ("r", Rope),
+        ("tokens", c_i64), ("hq", c_i32), ("hk", c_i32),
+        ("q", c_vp), ("k", c_vp), ("v", c_vp), ("q_tok", c_i64), ("q_head", c_i64), ("k_tok", c_i64), ("k_head", c_i64), ("v_tok", c_i64),
+        ("v_head", c_i64),
+        ("q_out", c_vp),
+        ("kc", c_vp), ("vc", c_vp), ("kc_page", c_i64), ("kc_head", c_i64), ("kc_tok", c_i64), ("vc_page", c_i64), ("vc_head", c_i64),
+        ("vc_tok", c_i64),
+        ("table", c_vp), ("cu", c_vp), ("lens", c_vp), ("table_stride", c_i64),
+        ("k_scale", c_vp), ("v_scale", c_vp),
+        ("seqs", c_i32), ("table_w", c_i32), ("pages", c_i32), ("page", c_i32), ("cache_e4m3", c_i32), ("zero_tail", c_i32),
+    ]
+
+
 _PROTOS = {
     "hma_gemm_nt": [c_vp, C.POINTER(GemmNT)],
     "hma_gemm_tn": [c_vp, C.POINTER(GemmTN)],
@@ -238,6 +275,9 @@ _PROTOS = {
     "hma_chain_s_bwd": [c_vp, C.POINTER(ChainSBwd)],
     "hma_chain_t_bwd": [c_vp, C.POINTER(ChainTBwd)],
     "hma_chain_ab_fwd": [c_vp, C.POINTER(ChainABFwd)],
+    "hma_qk_rope_fwd": [c_vp, C.POINTER(QkRope)],
+    "hma_qk_rope_bwd": [c_vp, C.POINTER(QkRope)],
+    "hma_kv_append": [c_vp, C.POINTER(KvAppend)],
     "hma_zero_f32": [c_vp, c_vp, c_i64],
     "hma_abi_version": [],
 }

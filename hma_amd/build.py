@@ -9,8 +9,11 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libhma_hip.so")
-SOURCES = ["gemm.hip", "norm.hip", "attn_spatial.hip", "attn_temporal.hip", "embed.hip", "loss.hip", "optim.hip", "collate.hip", "diffusion.hip", "mar.hip", "mlp.hip", "chain.hip"]
+SOURCES = ["gemm.hip", "norm.hip", "attn_spatial.hip", "attn_temporal.hip", "embed.hip", "loss.hip", "optim.hip", "collate.hip", "diffusion.hip", "mar.hip", "mlp.hip", "chain.hip", "rope.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-comment"]
+# without packed fp32 instructions (hipcc forms them by itself from scalar code; the host pass warns that it does not know the feature)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FILE_FLAGS = {"rope.hip": NO_PACKED_F32, "attn_paged.hip": NO_PACKED_F32}
 
 
 def _hipcc() -> str:
@@ -37,7 +40,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         path = os.path.join(CSRC, src)
         if force or _stale(obj, [path] + headers):
-            cmd = [hipcc, *FLAGS, "-c", path, "-o", obj]
+            cmd = [hipcc, *FLAGS, *FILE_FLAGS.get(src, []), "-c", path, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
             subprocess.run(cmd, check=True)

@@ -6,14 +6,17 @@ eager / CPU fallback anywhere in this package.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
-from typing import Optional
+import math
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import (A_BF16, A_BF16_AFFINE, A_F32, EPI_ATOMIC_F32, EPI_BF16, EPI_DGELU, EPI_DSILU, EPI_F32, EPI_GELU2,
-                   EPI_RESID, EPI_SILU2, ChainABFwd, ChainABwd, ChainAFwd, ChainBFwd, ChainSBwd, ChainTBwd, GemmNT, GemmTN, MlpBwd, MlpFwd, ReadoutCE)
+                   EPI_RESID, EPI_SILU2, ChainABFwd, ChainABwd, ChainAFwd, ChainBFwd, ChainSBwd, ChainTBwd, GemmNT, GemmTN, KvAppend, MlpBwd, MlpFwd, QkRope,
+                   ReadoutCE)
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -313,3 +316,202 @@ def attn_temporal_bwd(qkv, o, d_o, batch: int, T: int, n_s: int, scale: float):
     dqkv = torch.empty_like(qkv)
     _lib.call("hma_attn_temporal_bwd", stream_ptr(), ptr(qkv), ptr(o), ptr(d_o), ptr(dqkv), batch, T, n_s, scale)
     return dqkv
+
+
+# ----------------------------------------------------------------------------------------------
+# positions, norms of queries / keys, paged cache (csrc/rope.hip)
+# ----------------------------------------------------------------------------------------------
+F8 = torch.float8_e4m3fn
+_DTYPE = {BF16: 0, torch.float16: 1, F32: 2}
+_NORM = {"none": 0, "rms": 1, "layer": 2}
+_QK_ROPE_WS_GROUPS = 1024
+
+
+def _device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
+    """Every tensor on `first`'s GPU; the context in which its kernels are launched (nothing where that GPU is the current one)."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise RuntimeError("hma ops run on the HIP kernels only (got a %s tensor)" % dev.type)
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """(tokens, heads, d) with contiguous 16-byte aligned rows: t itself, or a contiguous copy where its strides are others."""
+    s0, s1, s2 = t.stride()
+    m = 16 // t.element_size() - 1
+    return t if s2 == 1 and not ((s0 | s1) & m) and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0, trained: int = 8192, slow: float = 1.0,
+               fast: float = 32.0, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(frequencies, float64 (rot / 2,) radians per position, amplitude) of rotary positions: base ** (-2 i / rot), for contexts `factor`
+    times the `trained` length
+      "linear": every frequency divided by the factor;
+      "base":   the base raised so that the slowest pair is slowed by the factor and the fastest is not;
+      "parts":  pairs that turn at most `slow` times over the trained length divided by the factor, those that turn `fast` times or more
+                left, a linear ramp between; the amplitude is 1 + 0.1 ln(factor)."""
+    _need(rot > 0 and rot % 2 == 0 and base > 1 and factor > 0 and trained > 0 and fast > slow, "rope_freqs: rot even and positive, base > 1, factor > 0, fast > slow")
+    _need(scaling in ("none", "linear", "base", "parts"), f"rope_freqs: scaling {scaling!r}")
+    if scaling == "base" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+    amplitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        f = f * (keep + (1 - keep) / factor)
+        amplitude = 1.0 + 0.1 * math.log(factor) if factor > 1 else 1.0
+    return f.to(device), amplitude
+
+
+def _fill_rope(r, dtype, d: int, tokens: int, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps) -> None:
+    rot = 0
+    if freqs is not None:
+        _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and 2 * freqs.numel() <= d,
+              "freqs: float64 (rot / 2,) contiguous, rot <= head size")
+        rot = 2 * freqs.numel()
+        r.freqs = freqs.data_ptr()
+    r.n_axes = 1
+    if positions is not None and rot:
+        _need(positions.dtype in (torch.int64, torch.int32) and positions.dim() in (1, 2) and positions.shape[-1] == tokens and
+              (tokens <= 1 or positions.stride(-1) == 1), "positions: int64 or int32, (tokens,) or (axes, tokens), contiguous over the tokens")
+        r.positions, r.pos_64 = positions.data_ptr(), positions.dtype == torch.int64
+        if positions.dim() == 2:
+            _need(positions.shape[0] >= 1 and (axes is not None or positions.shape[0] == 1) and (positions.shape[0] == 1 or positions.stride(0) >= tokens),
+                  "positions of several axes need `axes` and rows that do not overlap")
+            r.n_axes, r.pos_stride = positions.shape[0], positions.stride(0)
+    if axes is not None and rot:
+        _need(axes.dtype == torch.int32 and axes.shape == freqs.shape and axes.is_contiguous(), "axes: int32 (rot / 2,) contiguous")
+        r.axes = axes.data_ptr()
+    _need(norm in _NORM, f"norm {norm!r}: none, rms or layer")
+    wt = None
+    for w in (q_weight, q_bias, k_weight, k_bias):
+        if w is not None:
+            _need(norm != "none" and w.shape == (d,) and w.is_contiguous() and w.dtype in (F32, dtype) and wt in (None, w.dtype),
+                  "norm weights: (head size,) contiguous, all fp32 or all of the rows' type, with a norm")
+            wt = w.dtype
+    _need(norm == "layer" or (q_bias is None and k_bias is None), "a bias goes with norm 'layer'")
+    r.q_w, r.q_b, r.k_w, r.k_b = ptr(q_weight), ptr(q_bias), ptr(k_weight), ptr(k_bias)
+    r.w_f32 = wt in (None, F32)
+    r.d, r.rot, r.interleaved, r.norm, r.dtype, r.eps, r.amplitude = d, rot, bool(interleaved), _NORM[norm], _DTYPE[dtype], eps, amplitude
+
+
+def _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps):
+    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and q.dtype == k.dtype and q.dtype in _DTYPE,
+          "q (tokens, heads, d) and k (tokens, kv heads, d) of one type: bf16, fp16 or fp32")
+    _need(freqs is None or positions is not None, "a rotation needs positions")
+    q, k = _rows16(q), _rows16(k)
+    tokens, p.hq, d = q.shape
+    p.tokens, p.hk = tokens, k.shape[1]
+    _fill_rope(p.r, q.dtype, d, tokens, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+    p.q, p.k = q.data_ptr(), k.data_ptr()
+    p.q_tok, p.q_head, _ = q.stride()
+    p.k_tok, p.k_head, _ = k.stride()
+    return q, k
+
+
+def qk_rope_fwd(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor], *, axes: Optional[torch.Tensor] = None,
+                interleaved: bool = False, amplitude: float = 1.0, norm: str = "none", q_weight=None, q_bias=None, k_weight=None, k_bias=None,
+                eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norm of each head of q (tokens, heads, d) and k (tokens, kv heads, d) -- none, "rms" or "layer", weights (d,) -- and the rotation of
+    its first 2 * len(freqs) values by positions * freqs, in one pass (hma_qk_rope_fwd).  bf16, fp16 or fp32; d a multiple of 8 up to 256;
+    views of a packed projection need no copy.  positions (tokens,) or (axes, tokens) with `axes` int32 naming each pair's axis.  Returns
+    contiguous (q, k)."""
+    p = QkRope()
+    with _device(q, k, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias):
+        qr, kr = _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        p.q_out, p.k_out = qo.data_ptr(), ko.data_ptr()
+        _lib.call("hma_qk_rope_fwd", stream_ptr(), C.byref(p))
+    return qo, ko
+
+
+def qk_rope_bwd(dy_q: torch.Tensor, dy_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor, freqs, positions, *, axes=None, interleaved: bool = False,
+                amplitude: float = 1.0, norm: str = "none", q_weight=None, q_bias=None, k_weight=None, k_bias=None, eps: float = 1e-5):
+    """(dq, dk, d q_weight, d q_bias, d k_weight, d k_bias) of qk_rope_fwd from its inputs and the gradients of its outputs; the weights'
+    gradients (None where there is no weight) are summed in 32 bits in a fixed order (hma_qk_rope_bwd)."""
+    p = QkRope()
+    with _device(q, k, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias, dy_q, dy_k):
+        _need(dy_q.shape == q.shape and dy_k.shape == k.shape and dy_q.dtype == q.dtype and dy_k.dtype == k.dtype, "gradients of the shapes and type of q and k")
+        qr, kr = _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        gq, gk = _rows16(dy_q), _rows16(dy_k)
+        p.dy_q, p.dy_k = gq.data_ptr(), gk.data_ptr()
+        p.dyq_tok, p.dyq_head, _ = gq.stride()
+        p.dyk_tok, p.dyk_head, _ = gk.stride()
+        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        dw = [None if w is None else torch.empty_like(w) for w in (q_weight, q_bias, k_weight, k_bias)]
+        p.dq, p.dk = dq.data_ptr(), dk.data_ptr()
+        p.dq_w, p.dq_b, p.dk_w, p.dk_b = (ptr(w) for w in dw)
+        ws = None
+        if any(w is not None for w in dw):
+            ws = torch.empty(_QK_ROPE_WS_GROUPS * 4 * q.shape[2], dtype=F32, device=q.device)
+            p.ws, p.ws_floats = ws.data_ptr(), ws.numel()
+        _lib.call("hma_qk_rope_bwd", stream_ptr(), C.byref(p))
+    return (dq, dk, *dw)
+
+
+def _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, dtype) -> None:
+    """The paged cache of hma_kv_append / hma_attn_paged_fwd: caches (pages, kv heads, page size, d), table int32 (sequences, pages of one)."""
+    pages, hk, page, d = k_cache.shape
+    _need(v_cache.shape == k_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.dtype in (dtype, F8) and page > 0,
+          "caches: (pages, kv heads, page size, d), both of the rows' type or both float8_e4m3fn")
+    _need(page_table.dim() == 2 and cu_seqlens.shape == (page_table.shape[0] + 1,) and kv_lens.shape == (page_table.shape[0],) and
+          page_table.dtype == cu_seqlens.dtype == kv_lens.dtype == torch.int32 and cu_seqlens.is_contiguous() and kv_lens.is_contiguous() and
+          (page_table.shape[1] <= 1 or page_table.stride(1) == 1), "page_table (sequences, n), cu_seqlens (sequences + 1,), kv_lens (sequences,): int32")
+    f8 = k_cache.dtype == F8
+    _need((k_scale is not None and v_scale is not None) if f8 else (k_scale is None and v_scale is None), "scales go with a float8_e4m3fn cache, and only with it")
+    if f8:
+        for s in (k_scale, v_scale):
+            _need(s.dtype == F32 and s.shape == (hk,) and s.is_contiguous(), "k_scale, v_scale: fp32 (kv heads,) contiguous")
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    p.kc, p.vc, p.cache_e4m3 = k_cache.data_ptr(), v_cache.data_ptr(), f8
+    p.kc_page, p.kc_head, p.kc_tok, one = k_cache.stride()
+    p.vc_page, p.vc_head, p.vc_tok, two = v_cache.stride()
+    _need(one == 1 and two == 1, "the caches' last dimension is contiguous")
+    p.table, p.cu, p.lens, p.table_stride = page_table.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.stride(0)
+    p.seqs, p.table_w, p.pages, p.page = page_table.shape[0], page_table.shape[1], pages, page
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+              kv_lens: torch.Tensor, *, q: Optional[torch.Tensor] = None, freqs=None, positions=None, axes=None, interleaved: bool = False,
+              amplitude: float = 1.0, norm: str = "none", q_weight=None, q_bias=None, k_weight=None, k_bias=None, eps: float = 1e-5,
+              k_scale=None, v_scale=None, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Puts the new keys (normed and rotated like qk_rope_fwd's) and values (tokens, kv heads, d) of a batch of sequences into the pages of
+    k_cache / v_cache (pages, kv heads, page size, d), in place and in one launch (hma_kv_append).  Rows cu_seqlens[b] .. cu_seqlens[b + 1]
+    belong to sequence b and become its last places: kv_lens[b] counts its tokens with the new ones; place p is row p % page size of page
+    page_table[b, p // page size].  positions None: a token's place.  float8_e4m3fn caches store x / scale[head].  With q (tokens, heads,
+    d): returns q normed and rotated (rows behind the last sequence zero; with q_out given they are left as they were).  A token without a
+    place (kv_lens too small, a page number outside the cache) is not stored.  Pages written by one call belong to one sequence each."""
+    p = KvAppend()
+    with _device(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, q, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias, k_scale,
+                 v_scale, q_out):
+        _need(k.dim() == 3 and v.shape == k.shape and k.dtype == v.dtype and k.dtype in (BF16, torch.float16), "k, v: (tokens, kv heads, d) of one type, bf16 or fp16")
+        tokens, p.hk, d = k.shape
+        p.tokens = tokens
+        _need(k_cache.dim() == 4 and k_cache.shape[1] == p.hk and k_cache.shape[3] == d, "caches of k's heads and head size")
+        _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, k.dtype)
+        _fill_rope(p.r, k.dtype, d, tokens, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        _need(q is not None or (q_weight is None and q_bias is None and q_out is None), "q's weights and output without q")
+        k, v = _rows16(k), _rows16(v)
+        p.k, p.v = k.data_ptr(), v.data_ptr()
+        p.k_tok, p.k_head, _ = k.stride()
+        p.v_tok, p.v_head, _ = v.stride()
+        if q is not None:
+            _need(q.dim() == 3 and q.shape[0] == tokens and q.shape[2] == d and q.dtype == k.dtype, "q: (tokens, heads, d) of k's type")
+            if q_out is None:
+                q_out, p.zero_tail = torch.empty(q.shape, dtype=q.dtype, device=q.device), 1
+            _need(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous(), "q_out: q's shape and type, contiguous")
+            q = _rows16(q)
+            p.q, p.q_out, p.hq = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            p.q_tok, p.q_head, _ = q.stride()
+        _lib.call("hma_kv_append", stream_ptr(), C.byref(p))
+    return q_out

@@ -12,7 +12,7 @@ st_transformer.py:24-27,104-113).  There is no CPU implementation: a CPU tensor 
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -371,5 +371,75 @@ def _(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, max_norm):
     return p.new_empty(p.shape, dtype=BF16)
 
 
+# ------------------------------------------------------------------------------------------------ positions and the paged cache
+@torch.library.custom_op("hma::qk_rope", mutates_args=(), device_types="cuda")
+def qk_rope(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor], axes: Optional[torch.Tensor],
+            interleaved: bool, amplitude: float, norm: str, q_weight: Optional[torch.Tensor], q_bias: Optional[torch.Tensor],
+            k_weight: Optional[torch.Tensor], k_bias: Optional[torch.Tensor], eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) with every head normed ("none", "rms", "layer") and its first 2 len(freqs) values rotated -- ops.qk_rope_fwd; differentiable
+    in q, k and the weights"""
+    return ops.qk_rope_fwd(q, k, freqs, positions, axes=axes, interleaved=interleaved, amplitude=amplitude, norm=norm, q_weight=q_weight,
+                           q_bias=q_bias, k_weight=k_weight, k_bias=k_bias, eps=eps)
+
+
+@qk_rope.register_fake
+def _(q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("hma::qk_rope_bwd", mutates_args=(), device_types="cuda")
+def qk_rope_bwd(dy_q: torch.Tensor, dy_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor],
+                positions: Optional[torch.Tensor], axes: Optional[torch.Tensor], interleaved: bool, amplitude: float, norm: str,
+                q_weight: Optional[torch.Tensor], q_bias: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                k_bias: Optional[torch.Tensor], eps: float) -> List[torch.Tensor]:
+    """[dq, dk] and the gradients of the weights that are given, in their order -- ops.qk_rope_bwd"""
+    d = ops.qk_rope_bwd(dy_q, dy_k, q, k, freqs, positions, axes=axes, interleaved=interleaved, amplitude=amplitude, norm=norm,
+                        q_weight=q_weight, q_bias=q_bias, k_weight=k_weight, k_bias=k_bias, eps=eps)
+    return [x for x in d if x is not None]
+
+
+@qk_rope_bwd.register_fake
+def _(dy_q, dy_k, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps):
+    return [q.new_empty(q.shape), k.new_empty(k.shape)] + [torch.empty_like(w) for w in (q_weight, q_bias, k_weight, k_bias) if w is not None]
+
+
+def _rope_setup(ctx, inputs, output):
+    q, k, freqs, positions, axes, interleaved, amplitude, norm, qw, qb, kw, kb, eps = inputs
+    ctx.save_for_backward(q, k, freqs, positions, axes, qw, qb, kw, kb)
+    ctx.args = (interleaved, amplitude, norm, eps)
+
+
+def _rope_backward(ctx, dy_q, dy_k):
+    q, k, freqs, positions, axes, *w = ctx.saved_tensors
+    interleaved, amplitude, norm, eps = ctx.args
+    d = iter(torch.ops.hma.qk_rope_bwd(dy_q.to(q.dtype), dy_k.to(k.dtype), q, k, freqs, positions, axes, interleaved, amplitude, norm, *w, eps))
+    dq, dk = next(d), next(d)
+    return (dq, dk, None, None, None, None, None, None, *(None if x is None else next(d) for x in w), None)
+
+
+qk_rope.register_autograd(_rope_backward, setup_context=_rope_setup)
+
+
+@torch.library.custom_op("hma::kv_append", mutates_args=("k_cache", "v_cache"), device_types="cuda")
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+              kv_lens: torch.Tensor, q: Optional[torch.Tensor], freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+              axes: Optional[torch.Tensor], interleaved: bool, amplitude: float, norm: str, q_weight: Optional[torch.Tensor],
+              q_bias: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], k_bias: Optional[torch.Tensor], eps: float,
+              k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> torch.Tensor:
+    """New keys (normed, rotated) and values into the pages of k_cache / v_cache, in place; returns q normed and rotated (an empty tensor
+    without q) -- ops.kv_append"""
+    out = ops.kv_append(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, q=q, freqs=freqs, positions=positions, axes=axes,
+                        interleaved=interleaved, amplitude=amplitude, norm=norm, q_weight=q_weight, q_bias=q_bias, k_weight=k_weight,
+                        k_bias=k_bias, eps=eps, k_scale=k_scale, v_scale=v_scale)
+    return k.new_empty(0) if out is None else out
+
+
+@kv_append.register_fake
+def _(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, q, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias,
+      k_weight, k_bias, eps, k_scale, v_scale):
+    return k.new_empty(0) if q is None else q.new_empty(q.shape)
+
+
 OPS = ("linear", "linear_wgrad", "layer_norm", "attn_spatial", "attn_spatial_bwd", "attn_temporal", "attn_temporal_bwd", "mlp",
-       "mlp_bwd", "qknorm", "qknorm_bwd", "embed", "modulate", "readout_ce", "maskgit_step", "adamw")
+       "mlp_bwd", "qknorm", "qknorm_bwd", "embed", "modulate", "readout_ce", "maskgit_step", "adamw", "qk_rope",
+       "qk_rope_bwd", "kv_append")

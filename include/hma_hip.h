@@ -591,6 +591,61 @@ int hma_readout_ce(void* stream, const hma_readout_ce_t* p);
 /* n floats at p = 0 (captured in graphs in front of kernels that accumulate with atomics) */
 int hma_zero_f32(void* stream, float* p, int64_t n);
 
+/* ---- Positions, norms of queries / keys, and attention over a paged cache (no counterpart in the reference, whose positions are learned
+ * tables and whose decode recomputes the window).  Head sizes and counts are arguments here; element types are */
+enum { HMA_BF16 = 0, HMA_F16 = 1, HMA_F32 = 2 };
+enum { HMA_NORM_NONE = 0, HMA_NORM_RMS = 1, HMA_NORM_LAYER = 2 };
+
+/* The rotation and the norms that hma_qk_rope_fwd / _bwd and hma_kv_append share.  A row is one head of one token, d values:
+ *   y = R (u w + b),  u = x (NONE) | x / sqrt(mean x^2 + eps) (RMS) | (x - mean x) / sqrt(var x + eps) (LAYER);
+ * R turns pair i < rot / 2 -- values (2 i, 2 i + 1) if interleaved, else (i, i + rot / 2) -- by positions[axes[i]][token] * freqs[i]
+ * radians and multiplies it by `amplitude`; values behind rot pass.  d % 8 == 0, d <= 256, rot even, 0 <= rot <= d.
+ * freqs: double [rot / 2]; axes: int32 [rot / 2] or NULL (one axis); positions: [n_axes] rows pos_stride apart of int64 (pos_64) or
+ * int32.  The angle is formed in 64 bits (exact to 1e-7 rad up to positions of 2^30).
+ * w / b of the norms ([d], NULL = 1 / 0; w_f32: fp32, else of the rows' type). */
+typedef struct {
+  const double* freqs; const int32_t* axes; const void* positions; int64_t pos_stride;
+  const void *q_w, *q_b, *k_w, *k_b;
+  int32_t d, rot, interleaved, norm, dtype, w_f32, pos_64, n_axes;
+  float eps, amplitude;
+} hma_rope_t;
+
+/* Forward: q [tokens][hq][d], k [tokens][hk][d] (strides in elements, the last one 1, rows 16-byte aligned) -> q_out, k_out
+ * contiguous.  Backward: gradients dy_q, dy_k (strided alike) -> dq, dk contiguous; dq_w .. dk_b ([d] of the weights' type, NULL = not
+ * wanted) are WRITTEN, summed in 32 bits in a fixed order through ws (HMA_QK_ROPE_WS_GROUPS * 4 * d floats, wanted only with them). */
+#define HMA_QK_ROPE_WS_GROUPS 1024
+typedef struct {
+  hma_rope_t r;
+  int64_t tokens; int32_t hq, hk;
+  const void *q, *k; int64_t q_tok, q_head, k_tok, k_head;
+  void *q_out, *k_out;
+  const void *dy_q, *dy_k; int64_t dyq_tok, dyq_head, dyk_tok, dyk_head;
+  void *dq, *dk; void *dq_w, *dq_b, *dk_w, *dk_b;
+  float* ws; int64_t ws_floats;
+} hma_qk_rope_t;
+int hma_qk_rope_fwd(void* stream, const hma_qk_rope_t* p);
+int hma_qk_rope_bwd(void* stream, const hma_qk_rope_t* p);
+
+/* Appends keys and values to a paged cache: row i of sequence b (rows cu[b] .. cu[b + 1], cu int32 [seqs + 1] from 0) goes to place
+ * lens[b] - (cu[b + 1] - cu[b]) + i of that sequence, i.e. lens (int32 [seqs]) counts the cached tokens WITH the new ones; place p is row
+ * p % page of page table[b][p / page].  k normed and rotated (r; positions NULL: the place), v as it is; both rounded once, to the
+ * rows' type or (cache_e4m3) to e4m3 after division by k_scale / v_scale [hk].  q (NULL = none): normed and rotated into q_out
+ * [tokens][hq][d].  Cache strides in elements, the values of a row contiguous, rows 16-byte (e4m3: 8-byte) aligned.  A row whose place is negative, behind the
+ * table, or in a page outside 0 .. pages - 1 is not stored.  Rows behind the last sequence (tokens > cu[seqs]) are not stored, their
+ * q_out is left or (zero_tail) cleared.  r.dtype: HMA_BF16 or HMA_F16. */
+typedef struct {
+  hma_rope_t r;
+  int64_t tokens; int32_t hq, hk;
+  const void *q, *k, *v; int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  void* q_out;
+  void *kc, *vc; int64_t kc_page, kc_head, kc_tok, vc_page, vc_head, vc_tok;
+  const int32_t *table, *cu, *lens; int64_t table_stride;
+  const float *k_scale, *v_scale;
+  int32_t seqs, table_w, pages, page, cache_e4m3, zero_tail;
+} hma_kv_append_t;
+int hma_kv_append(void* stream, const hma_kv_append_t* p);
+
+
 /* library identity, for the loader: returns 0x484d4104 */
 int hma_abi_version(void);
 
