@@ -207,6 +207,18 @@ class KvAppend(C.Structure):
     ]
 
 
+class AttnPaged(C.Structure):
+    _fields_ = [
+        ("q", c_vp), ("o", c_vp), ("lse", c_vp), ("kc", c_vp), ("vc", c_vp), ("table", c_vp), ("cu", c_vp), ("lens", c_vp), ("k_scale", c_vp),
+        ("v_scale", c_vp), ("ws", c_vp), ("ws_bytes", c_i64),
+        ("tokens", c_i64), ("q_tok", c_i64), ("q_head", c_i64), ("kc_page", c_i64), ("kc_head", c_i64), ("kc_tok", c_i64), ("vc_page", c_i64),
+        ("vc_head", c_i64), ("vc_tok", c_i64), ("table_stride", c_i64),
+        ("hq", c_i32), ("hk", c_i32), ("d", c_i32), ("dtype", c_i32), ("seqs", c_i32), ("table_w", c_i32), ("pages", c_i32), ("page", c_i32),
+        ("cache_e4m3", c_i32), ("causal", c_i32), ("window", c_i32), ("zero_tail", c_i32),
+        ("scale", c_f32), ("_pad", c_i32),
+    ]
+
+
 _PROTOS = {
     "hma_gemm_nt": [c_vp, C.POINTER(GemmNT)],
     "hma_gemm_tn": [c_vp, C.POINTER(GemmTN)],
@@ -278,6 +290,8 @@ _PROTOS = {
     "hma_qk_rope_fwd": [c_vp, C.POINTER(QkRope)],
     "hma_qk_rope_bwd": [c_vp, C.POINTER(QkRope)],
     "hma_kv_append": [c_vp, C.POINTER(KvAppend)],
+    "hma_attn_paged_ws": [C.POINTER(AttnPaged), C.POINTER(c_i64)],
+    "hma_attn_paged_fwd": [c_vp, C.POINTER(AttnPaged)],
     "hma_zero_f32": [c_vp, c_vp, c_i64],
     "hma_abi_version": [],
 }

@@ -9,7 +9,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libhma_hip.so")
-SOURCES = ["gemm.hip", "norm.hip", "attn_spatial.hip", "attn_temporal.hip", "embed.hip", "loss.hip", "optim.hip", "collate.hip", "diffusion.hip", "mar.hip", "mlp.hip", "chain.hip", "rope.hip"]
+SOURCES = ["gemm.hip", "norm.hip", "attn_spatial.hip", "attn_temporal.hip", "embed.hip", "loss.hip", "optim.hip", "collate.hip", "diffusion.hip", "mar.hip", "mlp.hip", "chain.hip", "rope.hip", "attn_paged.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-comment"]
 # without packed fp32 instructions (hipcc forms them by itself from scalar code; the host pass warns that it does not know the feature)
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -1,0 +1,775 @@
+// Attention of a batch's new tokens over a paged cache: from one token a sequence to whole prompts.
+//
+//   o = softmax(scale q K^T, over the keys the row sees) V,   lse = log sum exp of the scaled scores;
+// the new tokens are the last places of their sequence; a row at place p sees the keys 0 .. p (causal), p - window + 1 .. p (window), or
+// every key of its sequence (a frame whose tokens see each other).  A row that sees none: o = 0, lse = -inf.
+//
+// Rows.  The hq / hk query heads that share a key head are rows of one problem: row r of (sequence, key head) = token r / G, head r % G,
+// so a tile of rows reads each key once for the whole group and one decoded token of 8 shared heads is an 8-row problem.
+// Products.  S^T = K Q^T by v_mfma_f32_32x32x16: a lane then holds ONE row and 16 of 32 keys, the softmax is in-lane with one exchange
+// between the half-waves, and the packed probabilities are the B operand of O^T = V^T P^T as they lie (the contraction index is permuted
+// alike on both sides); V^T comes out of row-major LDS by transposing reads.  Scores, maxima, sums and O in 32 bits; probabilities are
+// rounded once to the rows' 16-bit type for the second product (2^-9 or 2^-12 relative, below what the output's own rounding does), the
+// sums take them unrounded.  The running maximum is raised only when a row exceeds it by 2^8: probabilities then reach 256 instead of 1,
+// which changes no relative rounding, and O is rescaled a few times instead of at every step.
+// Pages.  A lane looks up the page of one key, the loads take it by a lane exchange.  A key outside what the tile sees, or in a page
+// outside the cache, is loaded as zeros, so nothing that is not a sequence's own reaches a product.  e4m3 caches are widened to the rows'
+// type (exactly) on their way into LDS; the scales join the scores' factor and the output's.
+// Split.  Units of work -- (sequence, key head, row tile, key tile) in that order -- are dealt evenly over the workgroups, so one
+// long sequence among short ones fills the chip; a workgroup's first and last row tile may be shared, their (max, sum, O) go to a
+// workspace and a second launch joins them in unit order.  No atomics: the same bits every time.
+#include <atomic>
+
+#include "hma_common.h"
+#include "../../include/hma_hip.h"
+
+using namespace hma;
+
+namespace {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef short v4s16_t __attribute__((ext_vector_type(4)));
+typedef short v8s16_t __attribute__((ext_vector_type(8)));
+#define HMA_LDS(T) __attribute__((address_space(3))) T
+
+constexpr int TPB = 256, WAVES = 4;
+constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
+constexpr float LAZY = 8.0f;  // how far (in powers of two) a row may exceed its running maximum before O is rescaled
+constexpr int PAD = 16;       // LDS rows of D + 16 values: the 4 rows of a transposing read and the 8 rows of a 16-byte read hit 64 banks once
+
+struct Args {
+  const void* q;
+  void* o;
+  float* lse;
+  const uint8_t *kc, *vc;
+  const int32_t *table, *cu, *lens;
+  const float *k_scale, *v_scale;
+  float* part;     // [workgroup][first | last][row][D] then [..][row][max, sum]
+  int64_t* units;  // [seqs + 1] first unit of each sequence, then the units of a workgroup
+  int64_t tokens, q_tok, q_head, kc_page, kc_head, kc_tok, vc_page, vc_head, vc_tok, table_stride;  // cache strides in bytes
+  uint32_t page_mul;
+  int32_t page_shift, hq, hk, group, seqs, table_w, pages, page, causal, window, zero_tail, groups;
+  float scale;
+};
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T> struct Op;  // T: __bf16 or _Float16
+template <> struct Op<__bf16> {
+  static __device__ __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, bool hi) {  // two e4m3 values
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  }
+};
+template <> struct Op<_Float16> {
+  static __device__ __forceinline__ f32x16_t mfma(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const half2_t h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+  }
+  static __device__ __forceinline__ uint32_t widen(uint32_t w, bool hi) {
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
+};
+
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ------------------------------------------------------------------------------------- sequences, row tiles, units
+struct Seq {
+  int32_t row0, n, kv, len;  // first row of the batch, new tokens, keys that the table can hold, length
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int b) {
+  Seq s;
+  const int64_t c0 = min(max((int64_t)a.cu[b], (int64_t)0), a.tokens), c1 = min(max((int64_t)a.cu[b + 1], c0), a.tokens);
+  s.row0 = (int32_t)c0;
+  s.n = (int32_t)(c1 - c0);
+  s.len = a.lens[b];
+  const int64_t room = min((int64_t)a.table_w * a.page, (int64_t)0x7fff0000);
+  s.kv = a.pages > 0 ? (int32_t)min(max((int64_t)s.len, (int64_t)0), room) : 0;
+  return s;
+}
+__device__ __forceinline__ int row_tiles(const Args& a, const Seq& s, int tr) { return (int)(((int64_t)s.n * a.group + tr - 1) / tr); }
+// key tiles of a row tile: the most that any of the sequence's row tiles needs, one at least (a row that sees nothing is written too)
+__device__ __forceinline__ int key_tiles(const Args& a, const Seq& s, int tr, int tk) {
+  int t = (int)(((int64_t)s.kv + tk - 1) / tk);
+  if (a.window > 0) t = (int)min((int64_t)t, ((int64_t)a.window + tr / a.group + 2 + tk - 1) / tk + 1);
+  return max(t, 1);
+}
+// base[b] = units before sequence b, by the whole workgroup
+__device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t* wsum, int tr, int tk) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t carry = 0;
+  if (threadIdx.x == 0) base[0] = 0;
+  for (int b0 = 0; b0 < a.seqs; b0 += TPB) {
+    const int b = b0 + threadIdx.x;
+    int64_t v = 0;
+    if (b < a.seqs) {
+      const Seq s = seq_of(a, b);
+      v = (int64_t)a.hk * row_tiles(a, s, tr) * key_tiles(a, s, tr, tk);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t up = __shfl_up(v, o, 64);
+      if (lane >= o) v += up;
+    }
+    if (lane == 63) wsum[wave] = v;
+    __syncthreads();
+    int64_t before = carry;
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) before += wsum[w];
+      carry += wsum[w];
+    }
+    if (b < a.seqs) base[b + 1] = before + v;
+    __syncthreads();
+  }
+  __syncthreads();
+}
+
+// A row tile of a sequence: what its rows see
+struct Tile {
+  int32_t lo_min, lo_max, hi_min, hi_max, start;  // keys seen by any row: [lo_min, hi_max), by every row: [lo_max, hi_min); first key of key tile 0
+};
+__device__ __forceinline__ int32_t lo_of(const Args& a, const Seq& s, int tok) {
+  return a.window > 0 ? (int32_t)max((int64_t)0, (int64_t)s.len - s.n + tok - a.window + 1) : 0;
+}
+__device__ __forceinline__ int32_t hi_of(const Args& a, const Seq& s, int tok) {
+  return a.causal ? min(max(s.len - s.n + tok + 1, 0), s.kv) : s.kv;
+}
+__device__ __forceinline__ Tile tile_of(const Args& a, const Seq& s, int qt, int tr, int tk) {
+  const int r0 = qt * tr, r1 = (int)min((int64_t)r0 + tr, (int64_t)s.n * a.group) - 1;
+  const int t0 = r0 / a.group, t1 = r1 / a.group;
+  Tile t;
+  t.lo_min = lo_of(a, s, t0);
+  t.lo_max = lo_of(a, s, t1);
+  t.hi_min = hi_of(a, s, t0);
+  t.hi_max = hi_of(a, s, t1);
+  t.start = t.lo_min / tk * tk;
+  return t;
+}
+
+// ------------------------------------------------------------------------------------- one wave: 32 rows against blocks of 32 keys
+template <typename T, int D>
+struct Rows {
+  uint4 q[D / 16];
+  f32x16_t o[D / 32];
+  float m, l;       // running maximum (powers of two), sum of this half-wave's keys
+  int32_t lo, hi;   // keys that the row sees
+  bool live;
+  int64_t at;       // its row of o (tokens x heads)
+
+  __device__ __forceinline__ void begin(const Args& a, const Seq& s, int hk, int r) {
+    const int lane = threadIdx.x & 63;
+    live = r < (int64_t)s.n * a.group;
+    const int tok = live ? r / a.group : 0, h = hk * a.group + (live ? r - tok * a.group : 0);
+    at = (int64_t)(s.row0 + tok) * a.hq + h;
+    lo = live ? lo_of(a, s, tok) : 0;
+    hi = live ? hi_of(a, s, tok) : 0x7fffffff;
+    const uint16_t* p = (const uint16_t*)a.q + (int64_t)(s.row0 + tok) * a.q_tok + h * a.q_head + (lane >> 5) * 8;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) q[i] = live ? *reinterpret_cast<const uint4*>(p + i * 16) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  // scores of KB blocks of 32 keys; kt: their rows in LDS
+  template <int KB>
+  __device__ __forceinline__ void scores(const uint16_t* kt, f32x16_t (&s)[KB]) const {
+    const int lane = threadIdx.x & 63;
+    const uint16_t* p = kt + (lane & 31) * (D + PAD) + (lane >> 5) * 8;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[k][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s[k] = Op<T>::mfma(*reinterpret_cast<const uint4*>(p + k * 32 * (D + PAD) + i * 16), q[i], s[k]);
+    }
+  }
+  // what a row does not see, and keys without a page (bits of `bad`), out of the scores
+  template <int KB>
+  __device__ __forceinline__ void mask(f32x16_t (&s)[KB], int key0, uint64_t bad) const {
+    const int half = (threadIdx.x & 63) >> 5;
+    const uint32_t span = (uint32_t)max(hi - lo, 0);
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = k * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
+        const bool seen = (uint32_t)(key0 + i - lo) < span && !((bad >> i) & 1);
+        s[k][e] = seen ? s[k][e] : -INFINITY;
+      }
+  }
+  // s -> probabilities relative to the running maximum, packed as the second product's operand; c: the scores' factor in powers of two
+  template <int KB>
+  __device__ __forceinline__ void softmax(f32x16_t (&s)[KB], float c, uint4 (&p)[KB][2]) {
+    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        x0 = __builtin_fmaxf(__builtin_fmaxf(x0, s[k][e]), s[k][e + 1]);
+        x1 = __builtin_fmaxf(__builtin_fmaxf(x1, s[k][e + 2]), s[k][e + 3]);
+      }
+    float x = fmaxf(x0, x1);
+    x = fmaxf(x, __shfl_xor(x, 32, 64)) * c;
+    if (__ballot(x > m + LAZY)) {  // also where m is still -inf
+      const float up = fmaxf(m, x), f = m == -INFINITY ? 0.f : fast_exp2(m - up);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= f;
+      m = up;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
+    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        s[k][e] = fast_exp2(__builtin_fmaf(s[k][e], c, -sub));
+        s[k][e + 1] = fast_exp2(__builtin_fmaf(s[k][e + 1], c, -sub));
+        l0 += s[k][e];
+        l1 += s[k][e + 1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        p[k][h] = make_uint4(Op<T>::pack(s[k][8 * h], s[k][8 * h + 1]), Op<T>::pack(s[k][8 * h + 2], s[k][8 * h + 3]),
+                             Op<T>::pack(s[k][8 * h + 4], s[k][8 * h + 5]), Op<T>::pack(s[k][8 * h + 6], s[k][8 * h + 7]));
+    }
+    l += l0 + l1;
+  }
+  // o += V^T p; vt: the values' rows in LDS.  The transposing read gives lane (d = l & 31, half) the rows 4 half + {0..3} and those + 8 of
+  // 16 -- the order in which pack left a row's probabilities.
+  template <int KB>
+  __device__ __forceinline__ void values(const uint16_t* vt, const uint4 (&p)[KB][2]) {
+    const int lane = threadIdx.x & 63, i16 = lane & 15, g16 = lane >> 4;
+    const uint16_t* base = vt + (4 * (g16 >> 1) + (i16 >> 2)) * (D + PAD) + 16 * (g16 & 1) + 4 * (i16 & 3);
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint16_t* v = base + (k * 32 + h * 16) * (D + PAD) + i * 32;
+          const v4s16_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HMA_LDS(v4s16_t)*)v);
+          const v4s16_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HMA_LDS(v4s16_t)*)(v + 8 * (D + PAD)));
+          const v8s16_t w = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[i] = Op<T>::mfma(__builtin_bit_cast(uint4, w), p[k][h], o[i]);
+        }
+  }
+  // both half-waves' sums into each
+  __device__ __forceinline__ void finish() { l += __shfl_xor(l, 32, 64); }
+
+  // the rows' outputs: o / l, lse
+  __device__ __forceinline__ void write(const Args& a, float vs) const {
+    const int half = (threadIdx.x & 63) >> 5;
+    const float f = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);  // a NaN stays one
+    uint16_t* row = (uint16_t*)a.o + at * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {  // the half-waves trade quads: 16 contiguous bytes each
+        const uint32_t ax = Op<T>::pack(o[i][4 * g] * f, o[i][4 * g + 1] * f), ay = Op<T>::pack(o[i][4 * g + 2] * f, o[i][4 * g + 3] * f);
+        const uint32_t bx = Op<T>::pack(o[i][4 * g + 4] * f, o[i][4 * g + 5] * f), by = Op<T>::pack(o[i][4 * g + 6] * f, o[i][4 * g + 7] * f);
+        const auto r0 = __builtin_amdgcn_permlane32_swap(ax, bx, false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(ay, by, false, false);
+        if (live) *reinterpret_cast<uint4*>(row + i * 32 + 8 * g + 8 * half) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+      }
+    if (live && half == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+  }
+  // a share of a row tile: unnormalised, for the second launch
+  __device__ __forceinline__ void write_part(const Args& a, int64_t slot, int tr, int row) const {
+    const int half = (threadIdx.x & 63) >> 5;
+    float* p = a.part + (slot * tr + row) * D;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(p + i * 32 + 8 * g + 4 * half) = make_float4(o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]);
+      if (half == 0) {
+        float* ml = a.part + (int64_t)a.groups * 2 * tr * D + (slot * tr + row) * 2;
+        *reinterpret_cast<float2*>(ml) = make_float2(m, l);
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------- loads of a block of keys
+// A group of THREADS threads loads KEYS rows of 16-byte pieces; lane l of each wave knows the page and the place in it of key l.
+template <typename T, int D, bool F8, int KEYS, int THREADS>
+struct Loader {
+  static constexpr int BYTES = F8 ? D : 2 * D, CPR = BYTES / 16, RPI = THREADS / CPR, NI = RPI < KEYS ? KEYS / RPI : 1;
+  static_assert((KEYS % RPI == 0 || RPI == 2 * KEYS) && KEYS <= 64, "");  // 32-byte rows: 128 of the 256 threads load 64
+
+  static __device__ __forceinline__ void load(const uint8_t* c, int64_t page, int64_t tok, int pg, int off, int tid, uint4 (&r)[NI]) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = (i * RPI + tid / CPR) % KEYS;
+      const int p = __shfl(pg, row, 64), f = __shfl(off, row, 64);
+      r[i] = *reinterpret_cast<const uint4*>(c + (p < 0 ? 0 : p * page + f * tok) + (tid % CPR) * 16);
+    }
+  }
+  // `gaps`: some key has no page (pg < 0): zeros
+  static __device__ __forceinline__ void store(uint16_t* t, int pg, bool gaps, int tid, uint4 (&r)[NI]) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = (i * RPI + tid / CPR) % KEYS;  // more threads than pieces: the second half repeats the first's
+      if (gaps && __shfl(pg, row, 64) < 0) r[i] = make_uint4(0, 0, 0, 0);
+      uint16_t* p = t + row * (D + PAD) + (tid % CPR) * (F8 ? 16 : 8);
+      if (F8) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(Op<T>::widen(r[i].x, false), Op<T>::widen(r[i].x, true), Op<T>::widen(r[i].y, false), Op<T>::widen(r[i].y, true));
+        *reinterpret_cast<uint4*>(p + 8) = make_uint4(Op<T>::widen(r[i].z, false), Op<T>::widen(r[i].z, true), Op<T>::widen(r[i].w, false), Op<T>::widen(r[i].w, true));
+      } else {
+        *reinterpret_cast<uint4*>(p) = r[i];
+      }
+    }
+  }
+};
+
+// The page of key `key` of a sequence, -1 where the tile does not see it; `lost`: seen, but its page is none of the cache's
+struct Place {
+  int32_t pg, off;
+  bool lost;
+};
+__device__ __forceinline__ Place find_page(const Args& a, const int32_t* table, int key, const Tile& t) {
+  Place p = {-1, 0, false};
+  if (key >= t.lo_min && key < t.hi_max) {
+    const int32_t i = (int32_t)(((uint64_t)(uint32_t)key * a.page_mul) >> (31 + a.page_shift));
+    p.off = key - i * a.page;
+    const int32_t pg = table[i];
+    p.lost = pg < 0 || pg >= a.pages;
+    p.pg = p.lost ? -1 : pg;
+  }
+  return p;
+}
+
+// rows behind the last sequence
+template <int D>
+__device__ __forceinline__ void clear_tail(const Args& a) {
+  if (!a.zero_tail) return;
+  const int64_t end = min(max((int64_t)a.cu[a.seqs], (int64_t)0), a.tokens);
+  const int64_t rows = (a.tokens - end) * a.hq, n = rows * (D / 8), at = end * a.hq;
+  for (int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x; i < n; i += (int64_t)gridDim.x * TPB) {
+    *reinterpret_cast<uint4*>((uint16_t*)a.o + at * D + i * 8) = make_uint4(0, 0, 0, 0);
+    if (a.lse && i % (D / 8) == 0) a.lse[at + i / (D / 8)] = -INFINITY;
+  }
+}
+
+// first unit of this workgroup and the one behind its last; workgroups that run on one XCD (number % 8) take neighbouring shares
+__device__ __forceinline__ int share_of(int groups) {
+  const int b = blockIdx.x;
+  return groups % 8 == 0 ? (b & 7) * (groups >> 3) + (b >> 3) : b;
+}
+
+// ------------------------------------------------------------------------------------- few rows: the waves take different keys
+template <typename T, int D, bool F8, int KB>
+__global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
+  constexpr int TR = 32, KEYS = 32 * KB, TK = WAVES * KEYS, LD = D + PAD, NO = D / 32;
+  typedef Loader<T, D, F8, KEYS, 64> Ld;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int64_t wsum[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint16_t* tiles = (uint16_t*)smem;
+  uint16_t* mine = tiles + wave * KEYS * LD;
+  float* xch = (float*)smem;  // the waves' results on their way to wave 0
+  int64_t* base = (int64_t*)(smem + WAVES * KEYS * LD * 2);
+  clear_tail<D>(a);
+  if (a.seqs == 0) return;
+  unit_table(a, base, wsum, TR, TK);
+  const int64_t total = base[a.seqs], each = (total + a.groups - 1) / a.groups;
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i <= a.seqs; i += TPB) a.units[i] = base[i];
+    if (threadIdx.x == 0) a.units[a.seqs + 1] = each;
+  }
+  const int64_t g = share_of(a.groups), u0 = g * each, u1 = min(total, u0 + each);
+  if (u0 >= u1) return;
+  int b = 0;
+  for (int lo = 0, hi = a.seqs - 1; lo <= hi;) {  // the last sequence with base <= u0
+    const int mid = (lo + hi) >> 1;
+    if (base[mid] <= u0) b = mid, lo = mid + 1; else hi = mid - 1;
+  }
+  for (int64_t u = u0; u < u1;) {
+    while (base[b + 1] <= u) ++b;
+    const Seq s = seq_of(a, b);
+    const int nt = key_tiles(a, s, TR, TK), nq = row_tiles(a, s, TR);
+    const int64_t local = u - base[b], item = local / nt, first = u - (local - item * nt);
+    const int j0 = (int)(local - item * nt), j1 = (int)min((int64_t)nt, j0 + (u1 - u));
+    const int hk = (int)(item / nq), qt = (int)(item - (int64_t)hk * nq);
+    const Tile t = tile_of(a, s, qt, TR, TK);
+    const int32_t* table = a.table + b * a.table_stride;
+    const uint8_t *kc = a.kc + hk * a.kc_head, *vc = a.vc + hk * a.vc_head;
+    const float c = a.scale * LOG2E * (F8 ? a.k_scale[hk] : 1.0f);
+    Rows<T, D> r;
+    r.begin(a, s, hk, qt * TR + (lane & 31));
+
+    // key blocks of this wave: start + j TK + wave KEYS; only those that the tile sees
+    auto key_of = [&](int j) { return t.start + j * TK + wave * KEYS; };
+    int j = j0, je = j1;
+    while (j < je && key_of(j) + KEYS <= t.lo_min) ++j;
+    while (je > j && (int64_t)t.start + (int64_t)(je - 1) * TK + wave * KEYS >= t.hi_max) --je;
+    if (j < je) {
+      const int kl = lane & (KEYS - 1);
+      Place now = find_page(a, table, key_of(j) + kl, t), next = now;
+      uint4 kr[Ld::NI], vr[Ld::NI];
+      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, lane, kr);
+      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, lane, vr);
+      if (j + 1 < je) next = find_page(a, table, key_of(j + 1) + kl, t);
+      for (; j < je; ++j) {
+        const int key0 = key_of(j);
+        const bool gaps = __ballot(now.pg < 0) != 0, more = j + 1 < je;
+        const uint64_t bad = __ballot(now.lost);
+        f32x16_t sc[KB];
+        uint4 p[KB][2];
+        Ld::store(mine, now.pg, gaps, lane, kr);
+        if (more) Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, lane, kr);
+        wave_lds_order();
+        r.template scores<KB>(mine, sc);
+        if (bad || key0 < t.lo_max || key0 + KEYS > t.hi_min) r.template mask<KB>(sc, key0, bad);
+        r.template softmax<KB>(sc, c, p);
+        wave_lds_order();
+        Ld::store(mine, now.pg, gaps, lane, vr);
+        if (more) {
+          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, lane, vr);
+          now = next;
+          if (j + 2 < je) next = find_page(a, table, key_of(j + 2) + kl, t);
+        }
+        wave_lds_order();
+        r.template values<KB>(mine, p);
+        wave_lds_order();
+      }
+    }
+    r.finish();
+    // waves 2, 3 -> 0, 1, then 1 -> 0
+    for (int step = 2; step >= 1; step >>= 1) {
+      __syncthreads();
+      float* x = xch + (wave & (step - 1)) * (NO * 16 + 2) * 64 + lane;
+      if (wave >= step && wave < 2 * step) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[(i * 16 + e) * 64] = r.o[i][e];
+        x[NO * 16 * 64] = r.m;
+        x[(NO * 16 + 1) * 64] = r.l;
+      }
+      __syncthreads();
+      if (wave < step) {
+        const float m2 = x[NO * 16 * 64], l2 = x[(NO * 16 + 1) * 64], mm = fmaxf(r.m, m2);
+        const float f1 = r.m == -INFINITY ? 0.f : fast_exp2(r.m - mm), f2 = m2 == -INFINITY ? 0.f : fast_exp2(m2 - mm);
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r.o[i][e] = r.o[i][e] * f1 + x[(i * 16 + e) * 64] * f2;
+        r.l = r.l * f1 + l2 * f2;
+        r.m = mm;
+      }
+    }
+    if (wave == 0) {
+      if (j0 == 0 && j1 == nt)
+        r.write(a, F8 ? a.v_scale[hk] : 1.0f);
+      else
+        r.write_part(a, g * 2 + (first < u0 ? 0 : 1), TR, lane & 31);
+    }
+    __syncthreads();
+    u += j1 - j0;
+  }
+}
+
+// ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 128
+template <typename T, int D, bool F8, bool SPLIT>
+__global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
+  constexpr int TR = 128, TK = 64, LD = D + PAD, BUF = 2 * TK * LD;
+  typedef Loader<T, D, F8, TK, TPB> Ld;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int64_t wsum[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint16_t* tiles = (uint16_t*)smem;  // [2][keys | values][TK][LD]
+  int64_t* base = (int64_t*)(smem + 2 * BUF * 2);
+  clear_tail<D>(a);
+  if (a.seqs == 0) return;
+  int64_t u0 = 0, u1 = 1, g = 0;
+  int b = 0, slot_qt = 0;
+  if (SPLIT) {
+    unit_table(a, base, wsum, TR, TK);
+    const int64_t total = base[a.seqs], each = (total + a.groups - 1) / a.groups;
+    if (blockIdx.x == 0) {
+      for (int i = tid; i <= a.seqs; i += TPB) a.units[i] = base[i];
+      if (tid == 0) a.units[a.seqs + 1] = each;
+    }
+    g = share_of(a.groups);
+    u0 = g * each;
+    u1 = min(total, u0 + each);
+    if (u0 >= u1) return;
+    for (int lo = 0, hi = a.seqs - 1; lo <= hi;) {
+      const int mid = (lo + hi) >> 1;
+      if (base[mid] <= u0) b = mid, lo = mid + 1; else hi = mid - 1;
+    }
+  } else {
+    // row tile number -> sequence: sequence b owns the numbers floor(cu[b] G / TR) + b up to the next one's, as many as it can need
+    const int64_t slot = (int64_t)gridDim.x / a.hk - 1 - blockIdx.x / a.hk;  // the last tiles of a sequence, which see most, first
+    int lo = 0, hi = a.seqs;  // the last b with first(b) <= slot
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)a.cu[mid] * a.group / TR + mid <= slot) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    if (b >= a.seqs) return;
+    slot_qt = (int)(slot - ((int64_t)a.cu[b] * a.group / TR + b));
+  }
+  for (int64_t u = u0; u < u1;) {
+    if (SPLIT)
+      while (base[b + 1] <= u) ++b;
+    const Seq s = seq_of(a, b);
+    const int nq = row_tiles(a, s, TR);
+    int nt, j0, j1, hk, qt;
+    int64_t first = 0;
+    Tile t;
+    if (SPLIT) {
+      nt = key_tiles(a, s, TR, TK);
+      const int64_t local = u - base[b], item = local / nt;
+      first = u - (local - item * nt);
+      j0 = (int)(local - item * nt);
+      j1 = (int)min((int64_t)nt, j0 + (u1 - u));
+      hk = (int)(item / nq);
+      qt = (int)(item - (int64_t)hk * nq);
+      t = tile_of(a, s, qt, TR, TK);
+    } else {
+      qt = slot_qt;
+      hk = blockIdx.x % a.hk;
+      if (qt < 0 || qt >= nq) return;
+      t = tile_of(a, s, qt, TR, TK);
+      j0 = 0;
+      nt = j1 = max((t.hi_max - t.start + TK - 1) / TK, 0);
+    }
+    const int32_t* table = a.table + b * a.table_stride;
+    const uint8_t *kc = a.kc + hk * a.kc_head, *vc = a.vc + hk * a.vc_head;
+    const float c = a.scale * LOG2E * (F8 ? a.k_scale[hk] : 1.0f);
+    Rows<T, D> r;
+    r.begin(a, s, hk, qt * TR + wave * 32 + (lane & 31));
+    // what this wave's 32 rows see (rows that are none see nothing)
+    const int w0 = qt * TR + wave * 32;
+    const bool any = w0 < (int64_t)s.n * a.group;
+    Tile w = t;
+    if (any) w = tile_of(a, s, qt * WAVES + wave, 32, TK);
+    const int je = min(j1, max((t.hi_max - t.start + TK - 1) / TK, 0));
+    int j = j0;
+    if (j < je) {
+      Place now = find_page(a, table, t.start + j * TK + lane, t), next = now;
+      uint4 kr[Ld::NI], vr[Ld::NI];
+      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, tid, kr);
+      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, tid, vr);
+      if (j + 1 < je) next = find_page(a, table, t.start + (j + 1) * TK + lane, t);
+      for (int buf = 0; j < je; ++j, buf ^= 1) {
+        uint16_t *kt = tiles + buf * BUF, *vt = kt + TK * LD;
+        const bool gaps = __ballot(now.pg < 0) != 0;
+        const uint64_t bad = __ballot(now.lost);
+        Ld::store(kt, now.pg, gaps, tid, kr);
+        Ld::store(vt, now.pg, gaps, tid, vr);
+        if (j + 1 < je) {
+          Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, tid, kr);
+          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, tid, vr);
+          now = next;
+          if (j + 2 < je) next = find_page(a, table, t.start + (j + 2) * TK + lane, t);
+        }
+        __syncthreads();  // one barrier a tile: the other buffer's readers passed the last one
+        const int key0 = t.start + j * TK;
+        if (any && key0 < w.hi_max && key0 + TK > w.lo_min) {
+          f32x16_t sc[2];
+          uint4 p[2][2];
+          r.template scores<2>(kt, sc);
+          if (bad || key0 < w.lo_max || key0 + TK > w.hi_min) r.template mask<2>(sc, key0, bad);
+          r.template softmax<2>(sc, c, p);
+          r.template values<2>(vt, p);
+        }
+      }
+    }
+    r.finish();
+    if (!SPLIT || (j0 == 0 && j1 == nt))
+      r.write(a, F8 ? a.v_scale[hk] : 1.0f);
+    else
+      r.write_part(a, g * 2 + (first < u0 ? 0 : 1), TR, wave * 32 + (lane & 31));
+    if (!SPLIT) return;
+    __syncthreads();  // the next row tile fills the buffers anew
+    u += j1 - j0;
+  }
+}
+
+// ------------------------------------------------------------------------------------- joining shared row tiles
+// One workgroup a (row tile, key head); D / 4 threads a row.
+template <typename T, int D>
+__global__ __launch_bounds__(TPB) void attn_join_kernel(const Args a, int tr, int tk) {
+  constexpr int TPR = D / 4, RPB = TPB / TPR;
+  const int64_t slot = blockIdx.x / a.hk;
+  const int hk = blockIdx.x % a.hk;
+  int lo = 0, hi = a.seqs;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int64_t)a.cu[mid] * a.group / tr + mid <= slot) lo = mid; else hi = mid - 1;
+  }
+  if (lo >= a.seqs) return;
+  const Seq s = seq_of(a, lo);
+  const int64_t qt = slot - ((int64_t)a.cu[lo] * a.group / tr + lo);
+  const int nq = row_tiles(a, s, tr), nt = key_tiles(a, s, tr, tk);
+  if (qt < 0 || qt >= nq) return;
+  const int64_t each = a.units[a.seqs + 1], u0 = a.units[lo] + ((int64_t)hk * nq + qt) * nt;
+  const int64_t g0 = u0 / each, g1 = (u0 + nt - 1) / each;
+  if (g0 == g1) return;  // one workgroup had it all and wrote it
+  const int rows = (int)min((int64_t)tr, (int64_t)s.n * a.group - qt * tr), d4 = threadIdx.x % TPR;
+  const float* ml = a.part + (int64_t)a.groups * 2 * tr * D;
+  const float vs = a.v_scale ? a.v_scale[hk] : 1.0f;
+  for (int row = threadIdx.x / TPR; row < rows; row += RPB) {
+    float m = -INFINITY;
+    // workgroup g's share of this row tile: its first one unless the tile begins inside g's units
+    for (int64_t g = g0; g <= g1; ++g) m = fmaxf(m, ml[((g * 2 + (u0 < g * each ? 0 : 1)) * tr + row) * 2]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t g = g0; g <= g1; ++g) {
+      const int64_t at = (g * 2 + (u0 < g * each ? 0 : 1)) * tr + row;
+      const float2 x = *reinterpret_cast<const float2*>(ml + at * 2);
+      const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + d4 * 4);
+      const float f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m);
+      l += x.y * f;
+      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+    }
+    const float f = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
+    const int64_t r = qt * tr + row, tok = r / a.group, at = (s.row0 + tok) * a.hq + hk * a.group + (r - tok * a.group);
+    *reinterpret_cast<uint2*>((uint16_t*)a.o + at * D + d4 * 4) = make_uint2(Op<T>::pack(o.x * f, o.y * f), Op<T>::pack(o.z * f, o.w * f));
+    if (d4 == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+  }
+}
+
+// ------------------------------------------------------------------------------------- host
+struct Plan {
+  bool few, split;
+  int tr, tk, groups;
+  int64_t slots, ws;
+};
+constexpr int CUS = 256;
+
+bool usable(const hma_attn_paged_t* p) {
+  if (!p || (p->d != 32 && p->d != 64 && p->d != 128) || (p->dtype != HMA_BF16 && p->dtype != HMA_F16)) return false;
+  if (p->hq < 1 || p->hk < 1 || p->hq > 4096 || p->hq % p->hk || p->tokens < 0 || p->tokens > 0x3fffffff / p->hq * 1LL) return false;
+  if (p->seqs < 0 || p->seqs > 4096 || p->table_w < 0 || p->pages < 0 || p->page < 1 || p->window < 0 || (p->window > 0 && !p->causal)) return false;
+  return p->scale > 0.f && p->scale < 3e38f;
+}
+// Rule: sequences with at most 32 rows (tokens x shared heads) on average take the kernel whose waves share the keys, others the one
+// whose waves share the rows; the latter is split along the keys only where its row tiles do not give every compute unit its two
+// workgroups twice over.
+Plan plan_of(const hma_attn_paged_t* p) {
+  Plan r;
+  const int64_t group = p->hq / p->hk, rows = p->tokens * group;
+  r.few = rows <= 32LL * p->seqs;
+  const int kb = p->d == 128 && !p->cache_e4m3 ? 1 : 2;
+  r.tr = r.few ? 32 : 128;
+  r.tk = r.few ? WAVES * 32 * kb : 64;
+  r.slots = rows / r.tr + p->seqs;
+  r.split = r.few || r.slots * p->hk < 4 * CUS;
+  // no more workgroups than units: row tiles x key tiles of the longest sequence that the table can hold
+  const int64_t most = ((int64_t)p->table_w * p->page + r.tk - 1) / r.tk;
+  const int64_t units = r.slots * p->hk * (most > 0 ? most : 1);
+  r.groups = (int)(units < 2 * CUS ? (units > 0 ? units : 1) : 2 * CUS);
+  r.ws = r.split ? (int64_t)r.groups * 2 * r.tr * (p->d + 2) * 4 + (p->seqs + 2) * 8 : 0;
+  return r;
+}
+
+// One attribute call per kernel and process and device: the most LDS that any call asks for
+template <auto Kern>
+int allow_lds() {
+  static std::atomic<uint64_t> done{0};  // a bit per device
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return HMA_EINVAL;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 2 * 64 * (128 + PAD) * 2 + 4097 * 8);
+  if (e != hipSuccess) return -(int)e;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
+template <typename T, int D, bool F8>
+int launch(hipStream_t st, const Args& a, const Plan& r) {
+  constexpr int KB = D == 128 && !F8 ? 1 : 2, LD = D + PAD;
+  const size_t units = (size_t)(a.seqs + 1) * 8;
+  if (r.few) {
+    const size_t lds = (size_t)WAVES * 32 * KB * LD * 2 + units;
+    if (const int rc = allow_lds<attn_few_kernel<T, D, F8, KB>>()) return rc;
+    hipLaunchKernelGGL((attn_few_kernel<T, D, F8, KB>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
+  } else {
+    const size_t lds = (size_t)2 * 2 * 64 * LD * 2 + (r.split ? units : 0);
+    if (r.split) {
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, true>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, true>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
+    } else {
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, false>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, false>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), lds, st, a);
+    }
+  }
+  HMA_CHECK_LAUNCH();
+  if (r.split) {
+    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), 0, st, a, r.tr, r.tk);
+    HMA_CHECK_LAUNCH();
+  }
+  return 0;
+}
+template <typename T, int D>
+int launch_f8(hipStream_t st, const Args& a, const Plan& r, bool e) {
+  return e ? launch<T, D, true>(st, a, r) : launch<T, D, false>(st, a, r);
+}
+template <typename T>
+int launch_d(hipStream_t st, const Args& a, const Plan& r, bool e, int d) {
+  return d == 128 ? launch_f8<T, 128>(st, a, r, e) : d == 64 ? launch_f8<T, 64>(st, a, r, e) : launch_f8<T, 32>(st, a, r, e);
+}
+
+}  // namespace
+
+extern "C" int hma_attn_paged_ws(const hma_attn_paged_t* p, int64_t* bytes) {
+  if (!usable(p) || !bytes) return HMA_EINVAL;
+  *bytes = plan_of(p).ws;
+  return 0;
+}
+
+extern "C" int hma_attn_paged_fwd(void* stream, const hma_attn_paged_t* p) {
+  if (!usable(p)) return HMA_EINVAL;
+  if (p->tokens == 0) return 0;
+  const bool e = p->cache_e4m3 != 0;
+  if (!p->q || !p->o || ((uintptr_t)p->q & 15) || ((uintptr_t)p->o & 15) || p->q_tok < 0 || p->q_head < 0 || (p->q_tok & 7) || (p->q_head & 7)) return HMA_EINVAL;
+  if (!p->cu || (p->seqs > 0 && (!p->lens || (p->table_w > 0 && !p->table))) || (e && (!p->k_scale || !p->v_scale))) return HMA_EINVAL;
+  Args a = {};
+  const int64_t es = e ? 1 : 2, st[6] = {p->kc_page, p->kc_head, p->kc_tok, p->vc_page, p->vc_head, p->vc_tok};
+  if (p->pages > 0) {
+    for (int i = 0; i < 6; ++i)
+      if (st[i] < 0 || ((st[i] * es) & 15)) return HMA_EINVAL;
+    if (!p->kc || !p->vc || ((uintptr_t)p->kc & 15) || ((uintptr_t)p->vc & 15)) return HMA_EINVAL;
+  }
+  const Plan r = plan_of(p);
+  if (r.split && (!p->ws || ((uintptr_t)p->ws & 15) || p->ws_bytes < r.ws)) return HMA_EINVAL;
+  if (r.slots * p->hk > 0x7fffffff) return HMA_EINVAL;
+  a.q = p->q; a.o = p->o; a.lse = p->lse; a.kc = (const uint8_t*)p->kc; a.vc = (const uint8_t*)p->vc;
+  a.table = p->table; a.cu = p->cu; a.lens = p->lens;
+  a.k_scale = e ? p->k_scale : nullptr;
+  a.v_scale = e ? p->v_scale : nullptr;
+  a.tokens = p->tokens; a.q_tok = p->q_tok; a.q_head = p->q_head; a.table_stride = p->table_stride;
+  a.kc_page = st[0] * es; a.kc_head = st[1] * es; a.kc_tok = st[2] * es; a.vc_page = st[3] * es; a.vc_head = st[4] * es; a.vc_tok = st[5] * es;
+  // key / page = (key * page_mul) >> (31 + page_shift) for every key < 2^31: page_mul = ceil(2^(31 + s) / page), 2^s >= page
+  while ((1LL << a.page_shift) < p->page) ++a.page_shift;
+  a.page_mul = (uint32_t)(((1ULL << (31 + a.page_shift)) + p->page - 1) / p->page);
+  a.hq = p->hq; a.hk = p->hk; a.group = p->hq / p->hk; a.seqs = p->seqs; a.table_w = p->table_w; a.pages = p->pages; a.page = p->page;
+  a.causal = p->causal; a.window = p->window; a.zero_tail = p->zero_tail; a.groups = r.groups; a.scale = p->scale;
+  a.part = (float*)p->ws;
+  a.units = r.split ? (int64_t*)((uint8_t*)p->ws + (int64_t)r.groups * 2 * r.tr * (p->d + 2) * 4) : nullptr;
+  return p->dtype == HMA_BF16 ? launch_d<__bf16>((hipStream_t)stream, a, r, e, p->d) : launch_d<_Float16>((hipStream_t)stream, a, r, e, p->d);
+}

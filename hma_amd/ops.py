@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import (A_BF16, A_BF16_AFFINE, A_F32, EPI_ATOMIC_F32, EPI_BF16, EPI_DGELU, EPI_DSILU, EPI_F32, EPI_GELU2,
-                   EPI_RESID, EPI_SILU2, ChainABFwd, ChainABwd, ChainAFwd, ChainBFwd, ChainSBwd, ChainTBwd, GemmNT, GemmTN, KvAppend, MlpBwd, MlpFwd, QkRope,
+                   EPI_RESID, EPI_SILU2, ChainABFwd, ChainABwd, ChainAFwd, ChainBFwd, ChainSBwd, ChainTBwd, AttnPaged, GemmNT, GemmTN, KvAppend, MlpBwd, MlpFwd, QkRope,
                    ReadoutCE)
 
 BF16 = torch.bfloat16
@@ -515,3 +515,38 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             p.q_tok, p.q_head, _ = q.stride()
         _lib.call("hma_kv_append", stream_ptr(), C.byref(p))
     return q_out
+
+
+def attn_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                   kv_lens: torch.Tensor, scale: float, *, causal: bool = True, window: int = 0, k_scale=None, v_scale=None,
+                   out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, lse) of the new tokens q (tokens, heads, d) of a batch of sequences over the paged cache that kv_append filled (the same
+    page_table, cu_seqlens and kv_lens): each is at its place and sees the places up to it (causal), the last `window` of them, or its whole
+    sequence (causal=False: a chunk whose tokens see each other, such as a frame).  bf16 or fp16, d 32, 64 or 128, heads a multiple of
+    the cache's; a cache of q's type or float8_e4m3fn with scales (hma_attn_paged_fwd).  lse fp32 (tokens, heads); a row that sees no key has o = 0,
+    lse = -inf, and so have rows behind the last sequence (with out / lse given those are left as they were)."""
+    p = AttnPaged()
+    with _device(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, out, lse):
+        _need(q.dim() == 3 and q.dtype in (BF16, torch.float16) and k_cache.dim() == 4 and k_cache.shape[3] == q.shape[2] and k_cache.shape[1] > 0 and
+              q.shape[1] % k_cache.shape[1] == 0, "q: (tokens, heads, d) bf16 or fp16, heads a multiple of the cache's, d the cache's")
+        if q.shape[2] not in (32, 64, 128):
+            raise NotImplementedError("attn_paged is built for heads of 32, 64 and 128")
+        _need(window >= 0 and (causal or window == 0), "a window goes with causal")
+        _need(0 < scale < 3e38, "scale > 0")
+        _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, q.dtype)
+        q = _rows16(q)
+        p.tokens, p.hq, p.d = q.shape
+        p.hk, p.dtype, p.causal, p.window, p.scale = k_cache.shape[1], _DTYPE[q.dtype], causal, window, scale
+        p.q_tok, p.q_head, _ = q.stride()
+        _need((out is None) == (lse is None), "out and lse together")
+        if out is None:
+            out, lse, p.zero_tail = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(q.shape[:2], dtype=F32, device=q.device), 1
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and lse.shape == q.shape[:2] and lse.dtype == F32 and
+              lse.is_contiguous(), "out: q's shape and type, lse: fp32 (tokens, heads), contiguous")
+        p.q, p.o, p.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
+        n = C.c_int64()
+        _lib.call("hma_attn_paged_ws", C.byref(p), C.byref(n))
+        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
+        p.ws, p.ws_bytes = ptr(ws), n.value
+        _lib.call("hma_attn_paged_fwd", stream_ptr(), C.byref(p))
+    return out, lse

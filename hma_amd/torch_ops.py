@@ -440,6 +440,20 @@ def _(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, q, freqs, positio
     return k.new_empty(0) if q is None else q.new_empty(q.shape)
 
 
+@torch.library.custom_op("hma::attn_paged", mutates_args=(), device_types="cuda")
+def attn_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+               kv_lens: torch.Tensor, scale: float, causal: bool, window: int, k_scale: Optional[torch.Tensor],
+               v_scale: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(o, lse) of a batch's new tokens over a paged cache -- ops.attn_paged_fwd (inference: no gradient)"""
+    return ops.attn_paged_fwd(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, scale, causal=causal, window=window, k_scale=k_scale,
+                              v_scale=v_scale)
+
+
+@attn_paged.register_fake
+def _(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, scale, causal, window, k_scale, v_scale):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=F32)
+
+
 OPS = ("linear", "linear_wgrad", "layer_norm", "attn_spatial", "attn_spatial_bwd", "attn_temporal", "attn_temporal_bwd", "mlp",
        "mlp_bwd", "qknorm", "qknorm_bwd", "embed", "modulate", "readout_ce", "maskgit_step", "adamw", "qk_rope",
-       "qk_rope_bwd", "kv_append")
+       "qk_rope_bwd", "kv_append", "attn_paged")

@@ -645,6 +645,28 @@ typedef struct {
 } hma_kv_append_t;
 int hma_kv_append(void* stream, const hma_kv_append_t* p);
 
+/* Attention of the new rows of a batch of sequences over a paged cache (the arguments of the same names as in hma_kv_append; the
+ * new rows' keys and values are in the cache already).  q [tokens][hq][d] (strides in elements, rows 16-byte aligned), d 32, 64 or 128,
+ * HMA_BF16 or HMA_F16; hq a multiple of hk, query head h reads key head h / (hq / hk); o [tokens][hq][d] contiguous, lse fp32
+ * [tokens][hq] or NULL.  Row i of sequence b is at place p = lens[b] - (cu[b + 1] - cu[b]) + i and sees the keys 0 .. p (causal), the
+ * last `window` of them (window > 0), or all of its sequence's lens[b] (not causal); keys in pages outside 0 .. pages - 1, or behind the table, are
+ * not seen.  o = softmax(scale q k) v, lse = log sum exp; a row that sees no key: o = 0, lse = -inf.  Cache rows that no row of
+ * a tile of rows sees are not read into any product, whatever they hold.  Rows behind the last sequence are left or (zero_tail) o = 0, lse = -inf.
+ * scale > 0; seqs <= 4096; cache strides in elements, rows 16-byte aligned.  ws: 16-byte aligned scratch of hma_attn_paged_ws bytes (from
+ * the same struct; pointers are not looked at), one for each call in flight.  No atomics: the same bits every time. */
+typedef struct {
+  const void* q; void* o; float* lse;
+  const void *kc, *vc;
+  const int32_t *table, *cu, *lens;
+  const float *k_scale, *v_scale;
+  void* ws; int64_t ws_bytes;
+  int64_t tokens, q_tok, q_head, kc_page, kc_head, kc_tok, vc_page, vc_head, vc_tok, table_stride;
+  int32_t hq, hk, d, dtype, seqs, table_w, pages, page, cache_e4m3, causal, window, zero_tail;
+  float scale; int32_t _pad;
+} hma_attn_paged_t;
+int hma_attn_paged_ws(const hma_attn_paged_t* p, int64_t* bytes);
+int hma_attn_paged_fwd(void* stream, const hma_attn_paged_t* p);
+
 
 /* library identity, for the loader: returns 0x484d4104 */
 int hma_abi_version(void);
