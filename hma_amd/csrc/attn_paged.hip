@@ -18,6 +18,7 @@
 // Split.  Units of work -- (sequence, key head, row tile, key tile) in that order -- are dealt evenly over the workgroups, so one
 // long sequence among short ones fills the chip; a workgroup's first and last row tile may be shared, their (max, sum, O) go to a
 // workspace and a second launch joins them in unit order.  No atomics: the same bits every time.
+#include <algorithm>
 #include <atomic>
 
 #include "hma_common.h"
@@ -107,7 +108,7 @@ __device__ __forceinline__ int key_tiles(const Args& a, const Seq& s, int tr, in
 }
 // base[b] = units before sequence b, by the whole workgroup
 __device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t* wsum, int tr, int tk) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t carry = 0;
   if (threadIdx.x == 0) base[0] = 0;
   for (int b0 = 0; b0 < a.seqs; b0 += TPB) {
@@ -133,6 +134,21 @@ __device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t
     __syncthreads();
   }
   __syncthreads();
+}
+
+// Row tile numbers: sequence b owns first_slot(b) .. first_slot(b + 1) - 1, at least as many as it needs, known without a sum over the
+// sequences.  The sequence of a number by the whole wave, 64 candidates a step.
+__device__ __forceinline__ int64_t first_slot(const Args& a, int b, int tr) { return (int64_t)a.cu[b] * a.group / tr + b; }
+__device__ __forceinline__ int seq_of_slot(const Args& a, int64_t slot, int tr) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = a.seqs;
+  while (n > 0) {
+    const int st = (n + 63) >> 6, i = (lane + 1) * st;
+    const int c = __popcll(__ballot(i <= n && first_slot(a, lo + min(i, n), tr) <= slot));
+    lo += c * st;
+    n = st == 1 ? 0 : min(st, n - c * st);
+  }
+  return lo;  // seqs: behind the last sequence
 }
 
 // A row tile of a sequence: what its rows see
@@ -383,7 +399,7 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
   typedef Loader<T, D, F8, KEYS, 64> Ld;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int64_t wsum[WAVES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint16_t* tiles = (uint16_t*)smem;
   uint16_t* mine = tiles + wave * KEYS * LD;
   float* xch = (float*)smem;  // the waves' results on their way to wave 0
@@ -496,7 +512,7 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
   typedef Loader<T, D, F8, TK, TPB> Ld;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int64_t wsum[WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint16_t* tiles = (uint16_t*)smem;  // [2][keys | values][TK][LD]
   int64_t* base = (int64_t*)(smem + 2 * BUF * 2);
   clear_tail<D>(a);
@@ -519,16 +535,10 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
       if (base[mid] <= u0) b = mid, lo = mid + 1; else hi = mid - 1;
     }
   } else {
-    // row tile number -> sequence: sequence b owns the numbers floor(cu[b] G / TR) + b up to the next one's, as many as it can need
     const int64_t slot = (int64_t)gridDim.x / a.hk - 1 - blockIdx.x / a.hk;  // the last tiles of a sequence, which see most, first
-    int lo = 0, hi = a.seqs;  // the last b with first(b) <= slot
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)a.cu[mid] * a.group / TR + mid <= slot) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
+    b = __builtin_amdgcn_readfirstlane(seq_of_slot(a, slot, TR));
     if (b >= a.seqs) return;
-    slot_qt = (int)(slot - ((int64_t)a.cu[b] * a.group / TR + b));
+    slot_qt = (int)(slot - first_slot(a, b, TR));
   }
   for (int64_t u = u0; u < u1;) {
     if (SPLIT)
@@ -609,47 +619,55 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------- joining shared row tiles
-// One workgroup a (row tile, key head); D / 4 threads a row.
+// A workgroup joins as many rows of a (row tile, key head) as its threads hold, D / 4 threads a row; blockIdx.y walks the tile's rows.  The
+// shares of a row are loaded eight at a time: the launch is short and all latency.
 template <typename T, int D>
 __global__ __launch_bounds__(TPB) void attn_join_kernel(const Args a, int tr, int tk) {
-  constexpr int TPR = D / 4, RPB = TPB / TPR;
+  constexpr int TPR = D / 4, RPB = TPB / TPR, AT = 8;
   const int64_t slot = blockIdx.x / a.hk;
-  const int hk = blockIdx.x % a.hk;
-  int lo = 0, hi = a.seqs;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int64_t)a.cu[mid] * a.group / tr + mid <= slot) lo = mid; else hi = mid - 1;
-  }
-  if (lo >= a.seqs) return;
-  const Seq s = seq_of(a, lo);
-  const int64_t qt = slot - ((int64_t)a.cu[lo] * a.group / tr + lo);
+  const int hk = blockIdx.x % a.hk, b = seq_of_slot(a, slot, tr);
+  if (b >= a.seqs) return;
+  const Seq s = seq_of(a, b);
+  const int64_t qt = slot - first_slot(a, b, tr), each = a.units[a.seqs + 1], base = a.units[b];
   const int nq = row_tiles(a, s, tr), nt = key_tiles(a, s, tr, tk);
   if (qt < 0 || qt >= nq) return;
-  const int64_t each = a.units[a.seqs + 1], u0 = a.units[lo] + ((int64_t)hk * nq + qt) * nt;
-  const int64_t g0 = u0 / each, g1 = (u0 + nt - 1) / each;
+  const int64_t u0 = base + ((int64_t)hk * nq + qt) * nt, g0 = u0 / each, g1 = (u0 + nt - 1) / each;
   if (g0 == g1) return;  // one workgroup had it all and wrote it
-  const int rows = (int)min((int64_t)tr, (int64_t)s.n * a.group - qt * tr), d4 = threadIdx.x % TPR;
+  const int rows = (int)min((int64_t)tr, (int64_t)s.n * a.group - qt * tr), d4 = threadIdx.x % TPR, row = blockIdx.y * RPB + threadIdx.x / TPR;
+  if (row >= rows) return;
   const float* ml = a.part + (int64_t)a.groups * 2 * tr * D;
   const float vs = a.v_scale ? a.v_scale[hk] : 1.0f;
-  for (int row = threadIdx.x / TPR; row < rows; row += RPB) {
-    float m = -INFINITY;
-    // workgroup g's share of this row tile: its first one unless the tile begins inside g's units
-    for (int64_t g = g0; g <= g1; ++g) m = fmaxf(m, ml[((g * 2 + (u0 < g * each ? 0 : 1)) * tr + row) * 2]);
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t g = g0; g <= g1; ++g) {
-      const int64_t at = (g * 2 + (u0 < g * each ? 0 : 1)) * tr + row;
-      const float2 x = *reinterpret_cast<const float2*>(ml + at * 2);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + d4 * 4);
-      const float f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m);
-      l += x.y * f;
-      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t g = g0; g <= g1; g += AT) {
+    float2 x[AT];
+    float4 v[AT];
+    float up = m;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {  // workgroup gi's share of this row tile: its first one unless the tile begins inside gi's units
+      const int64_t gi = min(g + i, g1), at = (gi * 2 + (u0 < gi * each ? 0 : 1)) * tr + row;
+      x[i] = *reinterpret_cast<const float2*>(ml + at * 2);
+      v[i] = *reinterpret_cast<const float4*>(a.part + at * D + d4 * 4);
     }
-    const float f = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
-    const int64_t r = qt * tr + row, tok = r / a.group, at = (s.row0 + tok) * a.hq + hk * a.group + (r - tok * a.group);
-    *reinterpret_cast<uint2*>((uint16_t*)a.o + at * D + d4 * 4) = make_uint2(Op<T>::pack(o.x * f, o.y * f), Op<T>::pack(o.z * f, o.w * f));
-    if (d4 == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) up = fmaxf(up, x[i].x);
+    const float f0 = m == -INFINITY ? 0.f : fast_exp2(m - up);
+    l *= f0;
+    o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      const float f = g + i > g1 || x[i].x == -INFINITY ? 0.f : fast_exp2(x[i].x - up);
+      if (g + i > g1) continue;
+      l = __builtin_fmaf(x[i].y, f, l);
+      o.x = __builtin_fmaf(v[i].x, f, o.x); o.y = __builtin_fmaf(v[i].y, f, o.y);
+      o.z = __builtin_fmaf(v[i].z, f, o.z); o.w = __builtin_fmaf(v[i].w, f, o.w);
+    }
+    m = up;
   }
+  const float f = l > 0.f ? vs / l : (l == 0.f ? 0.f : l);
+  const int64_t r = qt * tr + row, tok = r / a.group, at = (s.row0 + tok) * a.hq + hk * a.group + (r - tok * a.group);
+  *reinterpret_cast<uint2*>((uint16_t*)a.o + at * D + d4 * 4) = make_uint2(Op<T>::pack(o.x * f, o.y * f), Op<T>::pack(o.z * f, o.w * f));
+  if (d4 == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
 }
 
 // ------------------------------------------------------------------------------------- host
@@ -720,7 +738,8 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
   }
   HMA_CHECK_LAUNCH();
   if (r.split) {
-    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), 0, st, a, r.tr, r.tk);
+    const int most = (int)std::min<int64_t>(r.tr, a.tokens * a.group), per = TPB / (D / 4);
+    hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(r.slots * a.hk), (unsigned)((most + per - 1) / per)), dim3(TPB), 0, st, a, r.tr, r.tk);
     HMA_CHECK_LAUNCH();
   }
   return 0;

@@ -8,9 +8,11 @@
 // behind `rot` have C = 1, S = 0, so no lane branches.  R^T is the same with -S.
 //
 // Bound by the HBM bytes of the rows.  A lane holds 8 consecutive values of a row (16-byte loads and stores of 16-bit types), D / 8
-// lanes (rounded up to a power of two) hold a row, 64 lanes several heads.  What would bound it instead is the angles: a sine and a
-// cosine cost more than everything else that happens to a value, and every head of a token needs the same ones.  So a workgroup takes
-// a tile of tokens, its threads first compute the tile's C / S table once (about one angle per thread) into LDS, and the heads read it.
+// lanes (rounded up to a power of two) hold a row, 64 lanes several heads: a unit, one load a lane.  What would bound it instead is the
+// angles: a sine and a cosine cost more than everything else that happens to a value, and every head of a token needs the same ones.  So
+// a wave takes the tokens whose pairs are about 64 (four at D = 32, one at D = 128), computes one angle per lane into its own C / S table
+// in LDS and walks the tokens' heads with it.  Waves share nothing but the norms' weights, so there is one barrier in a launch; a wave
+// fetches its next units (and the next tokens' positions) before it works on the current ones.
 // Angles: position times frequency in 64 bits, reduced to a fraction of a turn there, rounded to 32 bits after that -- a 32-bit product
 // at position 10^6 is off by 0.03 rad.
 // Reductions: everything in 32 bits; each output is rounded once.
@@ -23,8 +25,8 @@ namespace {
 
 constexpr int TPB = 256;    // threads of a workgroup
 constexpr int WAVES = TPB / 64;
-constexpr int TABLE = 512;  // C and S values (tokens x D) of a tile: two per thread each
-constexpr int MAX_TT = 16;  // tokens of a tile
+constexpr int MAX_WT = 16;  // tokens of a wave's batch
+constexpr int MAX_GROUPS = 1024;
 
 struct Bf16 { uint16_t v; };
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -32,15 +34,17 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 template <typename T> struct Io;
 template <> struct Io<Bf16> {
   typedef uint4 raw;
-  static __device__ __forceinline__ raw load(const void* p, int64_t i) { return *reinterpret_cast<const uint4*>((const uint16_t*)p + i); }
+  static constexpr int SIZE = 2;
+  static __device__ __forceinline__ raw load(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
   static __device__ __forceinline__ void unpack(const raw& r, float* f) { unpack8(r, f); }
-  static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) { *reinterpret_cast<uint4*>((uint16_t*)p + i) = pack8(f); }
+  static __device__ __forceinline__ void store(uint8_t* p, const float* f) { *reinterpret_cast<uint4*>(p) = pack8(f); }
   static __device__ __forceinline__ float one(const void* p, int64_t i) { return from_bf16(((const uint16_t*)p)[i]); }
   static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((uint16_t*)p)[i] = to_bf16(v); }
 };
 template <> struct Io<_Float16> {
   typedef uint4 raw;
-  static __device__ __forceinline__ raw load(const void* p, int64_t i) { return *reinterpret_cast<const uint4*>((const _Float16*)p + i); }
+  static constexpr int SIZE = 2;
+  static __device__ __forceinline__ raw load(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
   static __device__ __forceinline__ void unpack(const raw& r, float* f) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -50,30 +54,31 @@ template <> struct Io<_Float16> {
       f[2 * i + 1] = (float)h[1];
     }
   }
-  static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) {
+  static __device__ __forceinline__ void store(uint8_t* p, const float* f) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const half2_t h = {(_Float16)f[2 * j], (_Float16)f[2 * j + 1]};
       w[j] = __builtin_bit_cast(uint32_t, h);
     }
-    *reinterpret_cast<uint4*>((_Float16*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   static __device__ __forceinline__ float one(const void* p, int64_t i) { return (float)((const _Float16*)p)[i]; }
   static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((_Float16*)p)[i] = (_Float16)v; }
 };
 template <> struct Io<float> {
   struct raw { float4 a, b; };
-  static __device__ __forceinline__ raw load(const void* p, int64_t i) {
-    const float4* q = reinterpret_cast<const float4*>((const float*)p + i);
+  static constexpr int SIZE = 4;
+  static __device__ __forceinline__ raw load(const uint8_t* p) {
+    const float4* q = reinterpret_cast<const float4*>(p);
     return raw{q[0], q[1]};
   }
   static __device__ __forceinline__ void unpack(const raw& r, float* f) {
     f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
     f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
   }
-  static __device__ __forceinline__ void store(void* p, int64_t i, const float* f) {
-    float4* q = reinterpret_cast<float4*>((float*)p + i);
+  static __device__ __forceinline__ void store(uint8_t* p, const float* f) {
+    float4* q = reinterpret_cast<float4*>(p);
     q[0] = make_float4(f[0], f[1], f[2], f[3]);
     q[1] = make_float4(f[4], f[5], f[6], f[7]);
   }
@@ -83,7 +88,7 @@ template <> struct Io<float> {
 
 // 8 values -> 8 e4m3 bytes, nearest even, clamped to the type's largest value (a NaN stays one)
 __device__ __forceinline__ float sat8(float x) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.f, 448.f); }
-__device__ __forceinline__ void store_e4m3(void* p, int64_t i, const float* f, float mul) {
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f, float mul) {
   uint2 w;
   int a = 0, b = 0;
   a = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[0] * mul), sat8(f[1] * mul), a, false);
@@ -92,7 +97,7 @@ __device__ __forceinline__ void store_e4m3(void* p, int64_t i, const float* f, f
   b = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[6] * mul), sat8(f[7] * mul), b, true);
   w.x = (uint32_t)a;
   w.y = (uint32_t)b;
-  *reinterpret_cast<uint2*>((uint8_t*)p + i) = w;
+  *reinterpret_cast<uint2*>(p) = w;
 }
 
 // Sum over the lg (1, 2, .. 32) lanes that hold a row, in each of them
@@ -110,23 +115,28 @@ __device__ __forceinline__ void wave_lds_order() {  // this wave's LDS writes be
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// What the three kernels share of their arguments
+// What the kernels share of their arguments
 struct Shape {
   const double* freqs;
   const int32_t* axes;
   const void* positions;
   const void* w[2][2];  // [q | k][weight | bias]
-  int64_t tokens, pos_stride;
-  int32_t hq, hk, d, rot, inter, norm, w_f32, pos64, n_axes, lg, hp, tt, passes, py;
+  int64_t tokens, pos_stride, batches;
+  int32_t hq, hk, d, rot, inter, norm, w_f32, pos64, n_axes, lg, hp, wt, passes, py;
   float eps, amp;
 };
 
+struct WaveLds {
+  float c[256], s[256];  // [token of the batch][d]
+  float xch[64 * 8];
+  int32_t page[MAX_WT], off[MAX_WT];
+};
 struct Lds {
-  float c[TABLE], s[TABLE];
   float w[2][2][256];
-  float xch[WAVES][64 * 8];
-  int32_t page[MAX_TT], off[MAX_TT];
-  int64_t pos[MAX_TT];
+  WaveLds wave[WAVES];
+};
+struct BwdLds : Lds {
+  float acc[WAVES][2][2][64 * 8];  // [wave][q | k][weight | bias]: each lane's 8 columns, parked while the wave works on the other tensor
 };
 
 __device__ __forceinline__ float weight_at(const Shape& a, const void* p, int i, bool is_bf16) {
@@ -146,36 +156,56 @@ __device__ __forceinline__ void stage_weights(const Shape& a, Lds& L) {
   }
 }
 
-// The tile's table: C and S of every token and value.  `own` = positions come from L.pos (already in LDS).
-__device__ __forceinline__ void stage_angles(const Shape& a, Lds& L, int64_t tok0, int nt, bool own) {
-  const int half = a.rot >> 1, hd = a.d >> 1;
-  for (int i = threadIdx.x; i < nt * hd; i += TPB) {
-    const int t = i / hd, p = i - t * hd;
-    float c = 1.f, s = 0.f;
-    int e0 = 2 * p, e1 = 2 * p + 1;  // where the pair's two values sit
-    if (p < half) {
-      double pos;
-      if (own) {
-        pos = (double)L.pos[t];
-      } else {
-        int ax = a.axes ? a.axes[p] : 0;
-        ax = min(max(ax, 0), a.n_axes - 1);
-        const int64_t at = ax * a.pos_stride + tok0 + t;
-        pos = a.pos64 ? (double)((const int64_t*)a.positions)[at] : (double)((const int32_t*)a.positions)[at];
-      }
-      double x = pos * (a.freqs[p] * 0.15915494309189533577);  // turns
-      x -= rint(x);
-      sincospif((float)(2.0 * x), &s, &c);
-      c *= a.amp;
-      s *= a.amp;
-      if (!a.inter) e0 = p, e1 = p + half;
+// The angles of a wave's batch: lane l computes those of pair numbers l and l + 64 of its wt * d / 2 (two only where d > 128)
+struct Angles {
+  double f[2];      // turns per position
+  int32_t t[2], e[2][2];  // token of the batch (-1: none), where the pair's values sit in the table
+  const uint8_t* pos[2];
+  bool turn[2];
+
+  __device__ __forceinline__ void begin(const Shape& a, int lane) {
+    const int half = a.rot >> 1, hd = a.d >> 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = lane + 64 * k;
+      t[k] = i < a.wt * hd ? i / hd : -1;
+      const int p = i % hd;
+      turn[k] = t[k] >= 0 && p < half;
+      f[k] = turn[k] ? a.freqs[p] * 0.15915494309189533577 : 0.0;
+      const int ax = turn[k] && a.axes ? min(max(a.axes[p], 0), a.n_axes - 1) : 0;
+      pos[k] = (const uint8_t*)a.positions + ax * a.pos_stride * (a.pos64 ? 8 : 4);
+      const bool inter = a.inter || !turn[k];
+      e[k][0] = max(t[k], 0) * a.d + (inter ? 2 * p : p);
+      e[k][1] = max(t[k], 0) * a.d + (inter ? 2 * p + 1 : p + half);
     }
-    float* C = L.c + t * a.d;
-    float* S = L.s + t * a.d;
-    C[e0] = c; C[e1] = c;
-    S[e0] = -s; S[e1] = s;
   }
-}
+  __device__ __forceinline__ void position(const Shape& a, int64_t tok0, double* at) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && a.wt * a.d <= 128) break;
+      const int64_t tok = tok0 + t[k];
+      at[k] = 0.0;
+      if (turn[k] && tok < a.tokens) at[k] = a.pos64 ? (double)((const int64_t*)pos[k])[tok] : (double)((const int32_t*)pos[k])[tok];
+    }
+  }
+  __device__ __forceinline__ void stage(const Shape& a, WaveLds& L, const double* at) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && a.wt * a.d <= 128) break;
+      if (t[k] < 0) continue;
+      float c = 1.f, s = 0.f;
+      if (turn[k]) {
+        double x = at[k] * f[k];
+        x -= rint(x);
+        sincospif((float)(2.0 * x), &s, &c);
+        c *= a.amp;
+        s *= a.amp;
+      }
+      L.c[e[k][0]] = c; L.c[e[k][1]] = c;
+      L.s[e[k][0]] = -s; L.s[e[k][1]] = s;
+    }
+  }
+};
 
 __device__ __forceinline__ void read8(const float* p, float* f) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
@@ -184,9 +214,10 @@ __device__ __forceinline__ void read8(const float* p, float* f) {
 }
 
 // y = x C + x[partner] S (sgn = -1: the transposed rotation) for the 8 values e0 .. e0 + 7 of each lane's row
+template <bool INTER>
 __device__ __forceinline__ void rotate(const Shape& a, float* xch, int lane, int e0, const float* x, const float* c, const float* s, float sgn, float* y) {
   float p[8];
-  if (a.inter) {
+  if (INTER) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] = x[e ^ 1];
   } else {
@@ -216,14 +247,15 @@ __device__ __forceinline__ void rotate(const Shape& a, float* xch, int lane, int
   for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(p[e] * sgn, s[e], x[e] * c[e]);
 }
 
-// mean (layer) and 1 / deviation of a row; lanes behind the row hold zeros
+// mean (layer) and 1 / deviation of a row; what lanes behind the row hold does not count
+template <int NORM>
 __device__ __forceinline__ void row_stats(const Shape& a, const float* x, bool in_row, float inv_d, float& mean, float& rstd) {
   mean = 0.f;
-  if (a.norm == HMA_NORM_LAYER) {
+  if (NORM == HMA_NORM_LAYER) {
     float t = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) t += x[e];
-    mean = row_sum(t, a.lg) * inv_d;
+    mean = row_sum(in_row ? t : 0.f, a.lg) * inv_d;
   }
   float q = 0.f;
 #pragma unroll
@@ -245,140 +277,204 @@ struct FwdArgs {
   int32_t seqs, table_w, pages, page, zero_tail;
 };
 
-// Sequence of a row: how many of cu[1 .. n] are <= row, by the whole wave (64 candidates a step)
-__device__ __forceinline__ int find_seq(const int32_t* cu, int n, int64_t row, int lane) {
-  int lo = 0;
-  while (n > 64) {
-    const int st = (n + 63) >> 6, i = (lane + 1) * st;
-    const int c = __popcll(__ballot(i <= n && cu[lo + min(i, n)] <= row));
-    lo += c * st;
-    n = min(st, n - c * st);
+// Where the batch's rows go: lane t finds the sequence and place of row tok0 + t.  `sample`: cu at every st-th sequence (lane + 1) * st.
+struct Target {
+  int32_t page, off;  // off -1: belongs to a sequence, has no place in the cache; -2: behind the last sequence
+  int64_t place;
+};
+__device__ __forceinline__ Target find_target(const FwdArgs& g, int64_t tok0, int nt, int lane, int st, int sample) {
+  int mine = 0;
+  for (int t = 0; t < nt; ++t) {  // how many of cu[1 .. seqs] are <= the row: 64 candidates a step
+    const int64_t row = tok0 + t;
+    const int c = __popcll(__ballot((lane + 1) * st <= g.seqs && sample <= row));
+    int lo = c * st, n = min(st, g.seqs - lo);
+    if (st == 1) n = 0;
+    while (n > 0) {
+      const int s2 = (n + 63) >> 6, i = (lane + 1) * s2;
+      const int k = __popcll(__ballot(i <= n && g.cu[lo + min(i, n)] <= row));
+      lo += k * s2;
+      n = s2 == 1 ? 0 : min(s2, n - k * s2);
+    }
+    if (lane == t) mine = lo;
   }
-  if (n <= 0) return lo;
-  return lo + __popcll(__ballot(lane < n && cu[lo + min(lane + 1, n)] <= row));
+  Target r = {-1, -2, 0};
+  if (lane < nt && mine < g.seqs) {
+    const int64_t row = tok0 + lane;
+    const int c0 = g.cu[mine], c1 = g.cu[mine + 1], len = g.lens[mine];
+    if (row >= c0) {
+      r.off = -1;
+      r.place = (int64_t)len - c1 + row;
+      const int64_t pi = r.place >= 0 ? r.place / g.page : g.table_w;
+      if (pi < g.table_w) {
+        r.page = g.table[mine * g.table_stride + pi];
+        if (r.page >= 0 && r.page < g.pages) r.off = (int32_t)(r.place - pi * g.page);
+      }
+    }
+  }
+  return r;
 }
 
-template <typename T, bool APPEND, bool F8>
-__global__ __launch_bounds__(TPB) void rope_fwd_kernel(const FwdArgs g) {
+// Addresses of a unit: the token and the first head of the group are the wave's, so all but a lane's head of the group and its columns is
+// scalar arithmetic.  `at` = heads of this tensor in front of the group (negative: the group begins before the tensor's first).
+struct Part {
+  const uint8_t* p;
+  int64_t tok, head, lane;  // bytes per token, per head, of this lane
+  __device__ __forceinline__ void begin(const void* base, int64_t tok_, int64_t head_, int size, int sub, int e) {
+    p = (const uint8_t*)base;
+    tok = tok_ * size;
+    head = head_ * size;
+    lane = sub * head + e * size;
+  }
+  __device__ __forceinline__ const uint8_t* of(int64_t t, int at) const { return p + t * tok + at * head; }
+};
+
+template <typename T, bool APPEND, bool F8, int NORM, bool INTER>
+__global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_fwd_kernel(const FwdArgs g) {
+  constexpr int U = 2, SZ = Io<T>::SIZE, CS = F8 ? 1 : SZ;  // units in flight, bytes of a value and of a cached one
   __shared__ Lds L;
   const Shape& a = g.s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tok0 = (int64_t)blockIdx.x * a.tt;
-  const int nt = (int)min((int64_t)a.tt, a.tokens - tok0);
-  // this wave's units: a unit is one token's group of hp heads; blockIdx.y takes a share of every token's groups
-  const int pp = (a.passes + a.py - 1) / a.py, p_lo = blockIdx.y * pp, np = min(pp, a.passes - p_lo);
-  if (np <= 0) return;
-  const int units = nt * np, per = (units + WAVES - 1) / WAVES, u_lo = wave * per, u_hi = min(units, u_lo + per);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  WaveLds& W = L.wave[wave];
+  // this wave: a share (1 / py) of the heads of batches gw / py, + the grid's stride, ...
+  const int gw = blockIdx.x * WAVES + wave, step = gridDim.x * WAVES / a.py;
+  const int share = gw % a.py, pp = (a.passes + a.py - 1) / a.py, p_lo = share * pp, np = min(pp, a.passes - p_lo);
+  int64_t batch = gw / a.py;
   const int dl = lane & (a.lg - 1), sub = lane / a.lg, e0 = dl * 8;
   const bool in_row = e0 < a.d;
-  const int heads = a.hq + a.hk + (APPEND ? a.hk : 0);
+  const int er = in_row ? e0 : 0, hqk = a.hq + a.hk, heads = hqk + (APPEND ? a.hk : 0);
   const float inv_d = 1.0f / (float)a.d;
+  const bool places = APPEND && !a.positions;
+  Part pq, pk, pv;
+  pq.begin(g.q, g.q_tok, g.q_head, SZ, sub, er);
+  pk.begin(g.k, g.k_tok, g.k_head, SZ, sub, er);
+  if (APPEND) pv.begin(g.v, g.v_tok, g.v_head, SZ, sub, er);
 
-  auto fetch = [&](int u) {
-    const int t = u / np, h = min((p_lo + u - t * np) * a.hp + sub, heads - 1);
-    const int64_t tok = tok0 + t;
-    const int e = in_row ? e0 : 0;
-    if (h < a.hq) return Io<T>::load(g.q, tok * g.q_tok + h * g.q_head + e);
-    if (!APPEND || h < a.hq + a.hk) return Io<T>::load(g.k, tok * g.k_tok + (h - a.hq) * g.k_head + e);
-    return Io<T>::load(g.v, tok * g.v_tok + (h - a.hq - a.hk) * g.v_head + e);
-  };
-  typename Io<T>::raw nx;
-  if (u_lo < u_hi) nx = fetch(u_lo);
-
-  if (APPEND) {
-    for (int t = wave; t < nt; t += WAVES) {
-      const int64_t row = tok0 + t;
-      const int b = find_seq(g.cu, g.seqs, row, lane);
-      int32_t page = -1, off = 0;
-      int64_t place = 0;
-      if (b < g.seqs && row >= g.cu[b]) {
-        place = (int64_t)g.lens[b] - g.cu[b + 1] + row;
-        const int64_t pi = place / g.page;
-        if (place >= 0 && pi < g.table_w) {
-          page = g.table[b * g.table_stride + pi];
-          if (page < 0 || page >= g.pages) page = -1;
-          off = (int32_t)(place - pi * g.page);
-        }
-        if (page < 0) off = -1;  // belongs to a sequence, has no place in the cache
-      } else {
-        off = -2;  // behind the last sequence
+  // the next U units from (token t of batch bt, group p) on; a unit behind the batch's last is loaded as that one
+  auto fetch = [&](int64_t bt, int t, int p, typename Io<T>::raw* r) {
+    const int64_t tok0 = bt * a.wt;
+    const int nt = (int)min((int64_t)a.wt, a.tokens - tok0);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t tok = tok0 + t;
+      const int h0 = (p_lo + p) * a.hp, h = h0 + sub;
+      const uint8_t* at = pk.of(tok, h0 - a.hq) + pk.lane;
+      if (h < a.hq) at = pq.of(tok, h0) + pq.lane;
+      if (APPEND && h >= hqk) at = pv.of(tok, h0 - hqk) + pv.lane;
+      if (h >= heads) at = pk.of(tok, 0) + er * SZ;
+      r[i] = Io<T>::load(at);
+      if (++p == np) {
+        if (t + 1 < nt) p = 0, ++t; else p = np - 1;
       }
-      if (lane == 0) L.page[t] = page, L.off[t] = off, L.pos[t] = place;
     }
+  };
+  const bool mine = np > 0 && batch < a.batches;
+  typename Io<T>::raw nx[U];
+  double pos[2] = {0.0, 0.0};
+  Angles an;
+  const int st = APPEND ? max((g.seqs + 63) >> 6, 1) : 1;
+  int sample = 0x7fffffff;
+  if (mine) {
+    fetch(batch, 0, 0, nx);
+    if (APPEND && (lane + 1) * st <= g.seqs) sample = g.cu[(lane + 1) * st];
+    an.begin(a, lane);
+    if (!places) an.position(a, batch * a.wt, pos);
+  }
+  if (NORM != HMA_NORM_NONE) {
+    stage_weights<T>(a, L);
     __syncthreads();
   }
-  stage_weights<T>(a, L);
-  stage_angles(a, L, tok0, nt, APPEND && !g.s.positions);
-  __syncthreads();
+  if (!mine) return;
 
-  int t_cur = -1;
-  bool first = true, k_cur = false;
+  int k_cur = -1;
   float c[8], s[8], w[8], b[8];
-  for (int u = u_lo; u < u_hi; ++u) {
-    const typename Io<T>::raw r = nx;
-    if (u + 1 < u_hi) nx = fetch(u + 1);
-    const int t = u / np, h = (p_lo + u - t * np) * a.hp + sub;
-    const bool is_q = h < a.hq, is_v = APPEND && h >= a.hq + a.hk, is_k = !is_q && !is_v;
-    if (t != t_cur) {
-      t_cur = t;
-      read8(L.c + t * a.d + (in_row ? e0 : 0), c);
-      read8(L.s + t * a.d + (in_row ? e0 : 0), s);
-    }
-    if (first || __ballot(is_k != k_cur)) {
-      first = false;
-      k_cur = is_k;
-      read8(&L.w[is_k][0][in_row ? e0 : 0], w);
-      read8(&L.w[is_k][1][in_row ? e0 : 0], b);
-    }
-    float x[8], y[8];
-    Io<T>::unpack(r, x);
-    if (!in_row) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    }
-    float n[8];
-    if (a.norm != HMA_NORM_NONE) {
-      float mean, rstd;
-      row_stats(a, x, in_row, inv_d, mean, rstd);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) n[e] = __builtin_fmaf((x[e] - mean) * rstd, w[e], b[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) n[e] = x[e];
-    }
-    rotate(a, L.xch[wave], lane, e0, n, c, s, 1.f, y);
-    if (!in_row || h >= heads) continue;
-    const int64_t tok = tok0 + t;
-    if (!APPEND) {
-      if (is_q)
-        Io<T>::store(g.q_out, (tok * a.hq + h) * a.d + e0, y);
-      else
-        Io<T>::store(g.k_out, (tok * a.hk + (h - a.hq)) * a.d + e0, y);
-      continue;
-    }
-    const int off = L.off[t];
-    if (is_q) {
-      if (off == -2) {
-        if (!g.zero_tail) continue;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = 0.f;
+  while (batch < a.batches) {
+    const int64_t tok0 = batch * a.wt, nb = batch + step;
+    const int nt = (int)min((int64_t)a.wt, a.tokens - tok0);
+    if (APPEND) {
+      const Target tg = find_target(g, tok0, nt, lane, st, sample);
+      if (lane < nt) W.page[lane] = tg.page, W.off[lane] = tg.off;
+      if (places) {
+        const double pl = (double)tg.place;
+        pos[0] = __shfl(pl, max(an.t[0], 0), 64);
+        pos[1] = __shfl(pl, max(an.t[1], 0), 64);
       }
-      Io<T>::store(g.q_out, (tok * a.hq + h) * a.d + e0, y);
-      continue;
     }
-    if (off < 0) continue;
-    const int64_t page = L.page[t];
-    const int hk = is_v ? h - a.hq - a.hk : h - a.hq;
-    void* dst = is_v ? g.vc : g.kc;
-    const int64_t at = is_v ? page * g.vc_page + hk * g.vc_head + off * g.vc_tok + e0 : page * g.kc_page + hk * g.kc_head + off * g.kc_tok + e0;
-    if (is_v) {
+    an.stage(a, W, pos);
+    wave_lds_order();
+    if (!places && nb < a.batches) an.position(a, nb * a.wt, pos);
+    int t_cur = -1;
+    for (int t = 0, p = 0; t < nt;) {
+      typename Io<T>::raw r[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e];
+      for (int i = 0; i < U; ++i) r[i] = nx[i];
+      {
+        int t2 = t, p2 = p + U;
+        while (p2 >= np && t2 < nt) p2 -= np, ++t2;
+        if (t2 < nt)
+          fetch(batch, t2, p2, nx);
+        else if (nb < a.batches)
+          fetch(nb, 0, 0, nx);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (t >= nt) break;
+        const int64_t tok = tok0 + t;
+        const int h0 = (p_lo + p) * a.hp, h = h0 + sub;
+        const bool is_q = h < a.hq, is_v = APPEND && h >= hqk, live = in_row && h < heads;
+        if (t != t_cur) {
+          t_cur = t;
+          read8(W.c + t * a.d + er, c);
+          read8(W.s + t * a.d + er, s);
+        }
+        if (NORM != HMA_NORM_NONE) {  // the weights of this group's rows: q's, k's, or both (a lane's own)
+          const int kind = h0 + a.hp <= a.hq ? 0 : h0 >= a.hq ? 1 : 2;
+          if (kind != k_cur) {
+            k_cur = kind;
+            read8(&L.w[!is_q][0][er], w);
+            read8(&L.w[!is_q][1][er], b);
+          }
+        }
+        float x[8], y[8], n[8];
+        Io<T>::unpack(r[i], x);
+        if (!APPEND || h0 < hqk) {  // (a group of values alone has neither norm nor rotation)
+          if (NORM != HMA_NORM_NONE) {
+            float mean, rstd;
+            row_stats<NORM>(a, x, in_row, inv_d, mean, rstd);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) n[e] = __builtin_fmaf((x[e] - mean) * rstd, w[e], b[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) n[e] = x[e];
+          }
+          rotate<INTER>(a, W.xch, lane, e0, n, c, s, 1.f, y);
+        }
+        if (!APPEND) {
+          uint8_t* dst = (uint8_t*)(is_q ? g.q_out : g.k_out) + (is_q ? (tok * a.hq + h0) * a.d : (tok * a.hk + h0 - a.hq) * a.d) * SZ + (sub * a.d + e0) * SZ;
+          if (live) Io<T>::store(dst, y);
+        } else {
+          const int off = __builtin_amdgcn_readfirstlane(W.off[t]), page = __builtin_amdgcn_readfirstlane(W.page[t]);
+          if (is_v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[e];
+          }
+          if (is_q && off == -2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = 0.f;
+          }
+          if (live && is_q && (off != -2 || g.zero_tail)) Io<T>::store((uint8_t*)g.q_out + (tok * a.hq + h0) * a.d * SZ + (sub * a.d + e0) * SZ, y);
+          if (live && !is_q && off >= 0) {
+            const int64_t ks = page * g.kc_page + off * g.kc_tok + (h0 - a.hq) * g.kc_head, vs = page * g.vc_page + off * g.vc_tok + (h0 - hqk) * g.vc_head;
+            uint8_t* dst = is_v ? (uint8_t*)g.vc + (vs + sub * g.vc_head + e0) * CS : (uint8_t*)g.kc + (ks + sub * g.kc_head + e0) * CS;
+            if (F8)
+              store_e4m3(dst, y, 1.0f / (is_v ? g.v_scale[h - hqk] : g.k_scale[h - a.hq]));
+            else
+              Io<T>::store(dst, y);
+          }
+        }
+        if (++p == np) p = 0, ++t;
+      }
     }
-    if (F8)
-      store_e4m3(dst, at, y, 1.0f / (is_v ? g.v_scale : g.k_scale)[hk]);
-    else
-      Io<T>::store(dst, at, y);
+    batch = nb;
   }
 }
 
@@ -388,131 +484,181 @@ struct BwdArgs {
   const void *q, *k, *gq, *gk;
   void *dq, *dk;
   float* part;  // [workgroup][q | k][weight | bias][d]
-  int64_t q_tok, q_head, k_tok, k_head, gq_tok, gq_head, gk_tok, gk_head, tiles;
+  int64_t q_tok, q_head, k_tok, k_head, gq_tok, gq_head, gk_tok, gk_head;
 };
 
 // dx of every row; the sums for the weights per workgroup (a lane adds its 8 columns over all its rows in registers, the workgroup adds
 // its lanes in a fixed order), so no atomics and the same bits every time.
-template <typename T>
-__global__ __launch_bounds__(TPB) void rope_bwd_kernel(const BwdArgs g) {
-  __shared__ Lds L;
+template <typename T, int NORM, bool INTER>
+__global__ __launch_bounds__(TPB, Io<T>::SIZE == 2 ? 3 : 2) void rope_bwd_kernel(const BwdArgs g) {
+  constexpr int U = 2, SZ = Io<T>::SIZE;
+  __shared__ BwdLds L;
   const Shape& a = g.s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  WaveLds& W = L.wave[wave];
   const int dl = lane & (a.lg - 1), sub = lane / a.lg, e0 = dl * 8;
   const bool in_row = e0 < a.d;
   const int er = in_row ? e0 : 0, heads = a.hq + a.hk, np = a.passes;
   const float inv_d = 1.0f / (float)a.d;
-  float dw[2][8], db[2][8];
+  float dw[8], db[8];  // this lane's columns of the tensor that its rows belong to now
+  bool acc_k = false;
+  if (NORM != HMA_NORM_NONE) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = db[0][e] = db[1][e] = 0.f;
-  stage_weights<T>(a, L);
-
-  for (int64_t tile = blockIdx.x; tile < g.tiles; tile += gridDim.x) {
-    const int64_t tok0 = tile * a.tt;
-    const int nt = (int)min((int64_t)a.tt, a.tokens - tok0);
-    const int units = nt * np, per = (units + WAVES - 1) / WAVES, u_lo = wave * per, u_hi = min(units, u_lo + per);
-    auto fetch = [&](int u, typename Io<T>::raw& x, typename Io<T>::raw& d) {
-      const int t = u / np, h = min((u - t * np) * a.hp + sub, heads - 1);
-      const int64_t tok = tok0 + t;
-      const bool is_q = h < a.hq;
-      x = is_q ? Io<T>::load(g.q, tok * g.q_tok + h * g.q_head + er) : Io<T>::load(g.k, tok * g.k_tok + (h - a.hq) * g.k_head + er);
-      d = is_q ? Io<T>::load(g.gq, tok * g.gq_tok + h * g.gq_head + er) : Io<T>::load(g.gk, tok * g.gk_tok + (h - a.hq) * g.gk_head + er);
-    };
-    typename Io<T>::raw nx, nd;
-    if (u_lo < u_hi) fetch(u_lo, nx, nd);
-    __syncthreads();  // the last tile's readers of the table are done
-    stage_angles(a, L, tok0, nt, false);
-    __syncthreads();
-    int t_cur = -1;
-    bool first = true, k_cur = false;
-    float c[8], s[8], w[8];
-    for (int u = u_lo; u < u_hi; ++u) {
-      const typename Io<T>::raw rx = nx, rd = nd;
-      if (u + 1 < u_hi) fetch(u + 1, nx, nd);
-      const int t = u / np, h = (u - t * np) * a.hp + sub;
-      const bool is_k = h >= a.hq, live = in_row && h < heads;
-      if (t != t_cur) {
-        t_cur = t;
-        read8(L.c + t * a.d + er, c);
-        read8(L.s + t * a.d + er, s);
-      }
-      if (first || __ballot(is_k != k_cur)) {
-        first = false;
-        k_cur = is_k;
-        read8(&L.w[is_k][0][er], w);
-      }
-      float x[8], d[8], y[8];
-      Io<T>::unpack(rx, x);
-      Io<T>::unpack(rd, d);
-      if (!live) {
+    for (int e = 0; e < 8; ++e) {
+      dw[e] = db[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.f, d[e] = 0.f;
-      }
-      rotate(a, L.xch[wave], lane, e0, d, c, s, -1.f, y);
-      if (a.norm != HMA_NORM_NONE) {
-        float mean, rstd;
-        row_stats(a, x, in_row, inv_d, mean, rstd);
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = (x[e] - mean) * rstd;
-          const float gu = y[e] * x[e];
-          dw[0][e] += is_k ? 0.f : gu;
-          dw[1][e] += is_k ? gu : 0.f;
-          db[0][e] += is_k ? 0.f : y[e];
-          db[1][e] += is_k ? y[e] : 0.f;
-          y[e] *= w[e];
-          s1 += y[e];
-          s2 = __builtin_fmaf(y[e], x[e], s2);
-        }
-        if (!in_row) s1 = s2 = 0.f;
-        s1 = a.norm == HMA_NORM_LAYER ? row_sum(s1, a.lg) * inv_d : 0.f;
-        s2 = row_sum(s2, a.lg) * inv_d;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = rstd * (y[e] - s1 - x[e] * s2);
-      }
-      if (!live) continue;
-      const int64_t tok = tok0 + t;
-      if (!is_k)
-        Io<T>::store(g.dq, (tok * a.hq + h) * a.d + e0, y);
-      else
-        Io<T>::store(g.dk, (tok * a.hk + (h - a.hq)) * a.d + e0, y);
+      for (int k = 0; k < 4; ++k) L.acc[wave][k >> 1][k & 1][lane * 8 + e] = 0.f;
     }
   }
-  if (!g.part) return;
-  // lanes of the same columns: sub groups first (by shuffles), then the waves through LDS
-  for (int kind = 0; kind < 2; ++kind)
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
+  auto park = [&]() {
+    float* pw = &L.acc[wave][acc_k][0][lane * 8];
+    float* pb = &L.acc[wave][acc_k][1][lane * 8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float v = kind ? (which ? db[1][e] : dw[1][e]) : (which ? db[0][e] : dw[0][e]);
-        for (int o = a.lg; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-        if (sub == 0) L.xch[wave][e0 + e] = v;  // e0 + 7 < 256
-      }
-      __syncthreads();
-      for (int e = threadIdx.x; e < a.d; e += TPB) {
-        float v = 0.f;
+    for (int e = 0; e < 8; ++e) {
+      pw[e] += dw[e];
+      dw[e] = 0.f;
+      if (NORM == HMA_NORM_LAYER) pb[e] += db[e], db[e] = 0.f;
+    }
+  };
+  int64_t batch = (int64_t)blockIdx.x * WAVES + wave;
+  const int64_t step = (int64_t)gridDim.x * WAVES;
+  Part pq, pk, gq, gk;
+  pq.begin(g.q, g.q_tok, g.q_head, SZ, sub, er);
+  pk.begin(g.k, g.k_tok, g.k_head, SZ, sub, er);
+  gq.begin(g.gq, g.gq_tok, g.gq_head, SZ, sub, er);
+  gk.begin(g.gk, g.gk_tok, g.gk_head, SZ, sub, er);
+
+  auto fetch = [&](int64_t bt, int t, int p, typename Io<T>::raw* x, typename Io<T>::raw* d) {
+    const int64_t tok0 = bt * a.wt;
+    const int nt = (int)min((int64_t)a.wt, a.tokens - tok0);
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) v += L.xch[k][e];
-        g.part[(((int64_t)blockIdx.x * 2 + kind) * 2 + which) * a.d + e] = v;
+    for (int i = 0; i < U; ++i) {
+      const int64_t tok = tok0 + t;
+      const int h0 = p * a.hp, h = h0 + sub;
+      const bool q = h < a.hq, none = h >= heads;
+      if (NORM != HMA_NORM_NONE) x[i] = Io<T>::load(none ? pk.of(tok, 0) + er * SZ : q ? pq.of(tok, h0) + pq.lane : pk.of(tok, h0 - a.hq) + pk.lane);
+      d[i] = Io<T>::load(none ? gk.of(tok, 0) + er * SZ : q ? gq.of(tok, h0) + gq.lane : gk.of(tok, h0 - a.hq) + gk.lane);
+      if (++p == np) {
+        if (t + 1 < nt) p = 0, ++t; else p = np - 1;
       }
     }
+  };
+  typename Io<T>::raw nx[U], nd[U];
+  double pos[2] = {0.0, 0.0};
+  Angles an;
+  if (batch < a.batches) {
+    fetch(batch, 0, 0, nx, nd);
+    an.begin(a, lane);
+    an.position(a, batch * a.wt, pos);
+  }
+  if (NORM != HMA_NORM_NONE) {
+    stage_weights<T>(a, L);
+    __syncthreads();
+  }
+  int k_cur = -1;
+  float c[8], s[8], w[8];
+  while (batch < a.batches) {
+    const int64_t tok0 = batch * a.wt, nb = batch + step;
+    const int nt = (int)min((int64_t)a.wt, a.tokens - tok0);
+    an.stage(a, W, pos);
+    wave_lds_order();
+    if (nb < a.batches) an.position(a, nb * a.wt, pos);
+    int t_cur = -1;
+    for (int t = 0, p = 0; t < nt;) {
+      typename Io<T>::raw rx[U], rd[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) rx[i] = nx[i], rd[i] = nd[i];
+      {
+        int t2 = t, p2 = p + U;
+        while (p2 >= np && t2 < nt) p2 -= np, ++t2;
+        if (t2 < nt)
+          fetch(batch, t2, p2, nx, nd);
+        else if (nb < a.batches)
+          fetch(nb, 0, 0, nx, nd);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (t >= nt) break;
+        const int64_t tok = tok0 + t;
+        const int h0 = p * a.hp, h = h0 + sub;
+        const bool is_k = h >= a.hq, live = in_row && h < heads;
+        const int kind = h0 + a.hp <= a.hq ? 0 : h0 >= a.hq ? 1 : 2;
+        if (t != t_cur) {
+          t_cur = t;
+          read8(W.c + t * a.d + er, c);
+          read8(W.s + t * a.d + er, s);
+        }
+        if (NORM != HMA_NORM_NONE && kind != k_cur) {
+          if (k_cur >= 0) park();
+          k_cur = kind;
+          acc_k = is_k;
+          read8(&L.w[is_k][0][er], w);
+        }
+        float d[8], y[8];
+        Io<T>::unpack(rd[i], d);
+        rotate<INTER>(a, W.xch, lane, e0, d, c, s, -1.f, y);
+        if (NORM != HMA_NORM_NONE) {
+          float x[8], mean, rstd;
+          Io<T>::unpack(rx[i], x);
+          row_stats<NORM>(a, x, in_row, inv_d, mean, rstd);
+          float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = (x[e] - mean) * rstd;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dw[e] += live ? y[e] * x[e] : 0.f;
+            if (NORM == HMA_NORM_LAYER) db[e] += live ? y[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            y[e] *= w[e];
+            s1 += y[e];
+            s2 = __builtin_fmaf(y[e], x[e], s2);
+          }
+          s1 = NORM == HMA_NORM_LAYER ? row_sum(in_row ? s1 : 0.f, a.lg) * inv_d : 0.f;
+          s2 = row_sum(in_row ? s2 : 0.f, a.lg) * inv_d;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = rstd * (y[e] - s1 - x[e] * s2);
+        }
+        uint8_t* dst = (uint8_t*)(is_k ? g.dk : g.dq) + (is_k ? (tok * a.hk + h0 - a.hq) * a.d : (tok * a.hq + h0) * a.d) * SZ + (sub * a.d + e0) * SZ;
+        if (live) Io<T>::store(dst, y);
+        if (++p == np) p = 0, ++t;
+      }
+    }
+    batch = nb;
+  }
+  if (NORM == HMA_NORM_NONE || !g.part) return;
+  park();
+  __syncthreads();
+  for (int i = threadIdx.x; i < 4 * a.d; i += TPB) {  // the lanes of the same columns, wave by wave
+    const int which = i / a.d, e = i - which * a.d, at = (e >> 3) * 8 + (e & 7);
+    float v = 0.f;
+    for (int k = 0; k < WAVES; ++k)
+      for (int j = 0; j < a.hp; ++j) v += L.acc[k][which >> 1][which & 1][j * a.lg * 8 + at];
+    g.part[(int64_t)blockIdx.x * 4 * a.d + i] = v;
+  }
 }
 
-// out[i] = sum over the workgroups' partial sums, i over [q | k][weight | bias][d]: 16 threads a value, in a fixed order
-__global__ __launch_bounds__(TPB) void rope_wsum_kernel(const float* part, int n, int width, void* qw, void* qb, void* kw, void* kb, int d, int w_f32, int bf16) {
-  __shared__ float sum[16][17];
+// out[i] = sum over the n workgroups' partial sums, i over [q | k][weight | bias][d]: 64 threads a value, each adding every 64th (8 loads
+// in flight), then in order
+__global__ __launch_bounds__(1024) void rope_wsum_kernel(const float* part, int n, int width, void* qw, void* qb, void* kw, void* kb, int d, int w_f32, int bf16) {
+  __shared__ float sum[64][17];
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4, i = blockIdx.x * 16 + col;
   float v = 0.f;
   if (i < width)
-    for (int k = row; k < n; k += 16) v += part[(int64_t)k * width + i];
+    for (int k = row; k < n; k += 512) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = k + 64 * j < n ? part[(int64_t)(k + 64 * j) * width + i] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v += x[j];
+    }
   sum[row][col] = v;
   __syncthreads();
   if (row || i >= width) return;
   v = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) v += sum[k][col];
+  for (int k = 0; k < 64; ++k) v += sum[k][col];
   const int which = i / d, e = i - which * d;
   void* out = which == 0 ? qw : which == 1 ? qb : which == 2 ? kw : kb;
   if (!out) return;
@@ -524,6 +670,43 @@ __global__ __launch_bounds__(TPB) void rope_wsum_kernel(const float* part, int n
     Io<_Float16>::put(out, e, v);
 }
 
+// Workgroups of a forward launch: a wave per (batch, share of the heads), at most what is resident (a wave then walks several batches)
+unsigned fwd_groups(const Shape& s) {
+  const int64_t want = (s.batches * s.py + WAVES - 1) / WAVES;
+  return (unsigned)(want < MAX_GROUPS || s.py > 1 ? want : MAX_GROUPS);
+}
+template <typename T, bool APPEND, bool F8, int NORM>
+void launch_fwd_n(hipStream_t st, const FwdArgs& g) {
+  if (g.s.inter)
+    hipLaunchKernelGGL((rope_fwd_kernel<T, APPEND, F8, NORM, true>), dim3(fwd_groups(g.s)), dim3(TPB), 0, st, g);
+  else
+    hipLaunchKernelGGL((rope_fwd_kernel<T, APPEND, F8, NORM, false>), dim3(fwd_groups(g.s)), dim3(TPB), 0, st, g);
+}
+template <typename T, bool APPEND, bool F8>
+void launch_fwd(hipStream_t st, const FwdArgs& g) {
+  if (g.s.norm == HMA_NORM_NONE)
+    launch_fwd_n<T, APPEND, F8, HMA_NORM_NONE>(st, g);
+  else if (g.s.norm == HMA_NORM_RMS)
+    launch_fwd_n<T, APPEND, F8, HMA_NORM_RMS>(st, g);
+  else
+    launch_fwd_n<T, APPEND, F8, HMA_NORM_LAYER>(st, g);
+}
+template <typename T, int NORM>
+void launch_bwd_n(hipStream_t st, const BwdArgs& g, unsigned groups) {
+  if (g.s.inter)
+    hipLaunchKernelGGL((rope_bwd_kernel<T, NORM, true>), dim3(groups), dim3(TPB), 0, st, g);
+  else
+    hipLaunchKernelGGL((rope_bwd_kernel<T, NORM, false>), dim3(groups), dim3(TPB), 0, st, g);
+}
+template <typename T>
+void launch_bwd(hipStream_t st, const BwdArgs& g, unsigned groups) {
+  if (g.s.norm == HMA_NORM_NONE)
+    launch_bwd_n<T, HMA_NORM_NONE>(st, g, groups);
+  else if (g.s.norm == HMA_NORM_RMS)
+    launch_bwd_n<T, HMA_NORM_RMS>(st, g, groups);
+  else
+    launch_bwd_n<T, HMA_NORM_LAYER>(st, g, groups);
+}
 int pow2_up(int v) {
   int p = 1;
   while (p < v) p <<= 1;
@@ -554,15 +737,15 @@ int fill_shape(Shape& s, const hma_rope_t& r, int32_t hq, int32_t hk, int64_t to
   s.passes = (hq + hk + extra_heads + s.hp - 1) / s.hp;
   s.eps = r.eps;
   s.amp = r.amplitude;
-  // tokens of a tile: as many as the table holds (one angle per thread), fewer where the chip would not be filled; then the heads of a
-  // token over several workgroups, a unit per wave.  1024 workgroups = four on each compute unit.
-  s.tt = TABLE / r.d;
-  if (s.tt > MAX_TT) s.tt = MAX_TT;
-  while (s.tt > 1 && (tokens + s.tt - 1) / s.tt < 1024) s.tt >>= 1;
+  // tokens of a wave's batch: as many as have 64 pairs together
+  s.wt = 128 / r.d;
+  if (s.wt > MAX_WT) s.wt = MAX_WT;
+  if (s.wt < 1) s.wt = 1;
+  s.batches = (tokens + s.wt - 1) / s.wt;
+  // few tokens: the heads of a batch over several waves (each computes the angles again), until there are 4096 -- four a SIMD
   s.py = 1;
-  const int most = (s.passes + WAVES - 1) / WAVES;
-  while (s.py < most && (tokens + s.tt - 1) / s.tt * s.py < 1024) s.py <<= 1;
-  if (s.py > most) s.py = most;
+  while (s.py < s.passes && s.batches * s.py < 4096) s.py <<= 1;
+  if (s.py > s.passes) s.py = s.passes;
   return 0;
 }
 
@@ -580,15 +763,12 @@ extern "C" int hma_qk_rope_fwd(void* stream, const hma_qk_rope_t* p) {
     return HMA_EINVAL;
   g.q = p->q; g.k = p->k; g.q_out = p->q_out; g.k_out = p->k_out;
   g.q_tok = p->q_tok; g.q_head = p->q_head; g.k_tok = p->k_tok; g.k_head = p->k_head;
-  const int64_t tiles = (p->tokens + g.s.tt - 1) / g.s.tt;
-  if (tiles > 0x7fffffff) return HMA_EINVAL;
-  const dim3 grid((unsigned)tiles, (unsigned)g.s.py);
   if (p->r.dtype == HMA_BF16)
-    hipLaunchKernelGGL((rope_fwd_kernel<Bf16, false, false>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
+    launch_fwd<Bf16, false, false>((hipStream_t)stream, g);
   else if (p->r.dtype == HMA_F16)
-    hipLaunchKernelGGL((rope_fwd_kernel<_Float16, false, false>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
+    launch_fwd<_Float16, false, false>((hipStream_t)stream, g);
   else
-    hipLaunchKernelGGL((rope_fwd_kernel<float, false, false>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
+    launch_fwd<float, false, false>((hipStream_t)stream, g);
   HMA_CHECK_LAUNCH();
   return 0;
 }
@@ -609,21 +789,21 @@ extern "C" int hma_qk_rope_bwd(void* stream, const hma_qk_rope_t* p) {
   g.part = sums ? p->ws : nullptr;
   g.q_tok = p->q_tok; g.q_head = p->q_head; g.k_tok = p->k_tok; g.k_head = p->k_head;
   g.gq_tok = p->dyq_tok; g.gq_head = p->dyq_head; g.gk_tok = p->dyk_tok; g.gk_head = p->dyk_head;
-  g.tiles = (p->tokens + g.s.tt - 1) / g.s.tt;
   // no tokens: no workgroup, and the sums over nothing are zero
-  const unsigned groups = (unsigned)(g.tiles < HMA_QK_ROPE_WS_GROUPS ? g.tiles : HMA_QK_ROPE_WS_GROUPS);
+  const int64_t want = (g.s.batches + WAVES - 1) / WAVES;
+  const unsigned groups = (unsigned)(want < HMA_QK_ROPE_WS_GROUPS ? want : HMA_QK_ROPE_WS_GROUPS);
   if (groups) {
     if (p->r.dtype == HMA_BF16)
-      hipLaunchKernelGGL((rope_bwd_kernel<Bf16>), dim3(groups), dim3(TPB), 0, (hipStream_t)stream, g);
+      launch_bwd<Bf16>((hipStream_t)stream, g, groups);
     else if (p->r.dtype == HMA_F16)
-      hipLaunchKernelGGL((rope_bwd_kernel<_Float16>), dim3(groups), dim3(TPB), 0, (hipStream_t)stream, g);
+      launch_bwd<_Float16>((hipStream_t)stream, g, groups);
     else
-      hipLaunchKernelGGL((rope_bwd_kernel<float>), dim3(groups), dim3(TPB), 0, (hipStream_t)stream, g);
+      launch_bwd<float>((hipStream_t)stream, g, groups);
     HMA_CHECK_LAUNCH();
   }
   if (sums) {
     const int width = 4 * p->r.d;
-    hipLaunchKernelGGL(rope_wsum_kernel, dim3((width + 15) / 16), dim3(TPB), 0, (hipStream_t)stream, p->ws, (int)groups, width, p->dq_w, p->dq_b,
+    hipLaunchKernelGGL(rope_wsum_kernel, dim3((width + 15) / 16), dim3(1024), 0, (hipStream_t)stream, p->ws, (int)groups, width, p->dq_w, p->dq_b,
                        p->dk_w, p->dk_b, p->r.d, p->r.w_f32, p->r.dtype == HMA_BF16);
     HMA_CHECK_LAUNCH();
   }
@@ -655,17 +835,12 @@ extern "C" int hma_kv_append(void* stream, const hma_kv_append_t* p) {
   g.table_stride = p->table_stride;
   g.kc_page = p->kc_page; g.kc_head = p->kc_head; g.kc_tok = p->kc_tok; g.vc_page = p->vc_page; g.vc_head = p->vc_head; g.vc_tok = p->vc_tok;
   g.seqs = p->seqs; g.table_w = p->table_w; g.pages = p->pages; g.page = p->page; g.zero_tail = p->zero_tail;
-  const dim3 grid((unsigned)((p->tokens + g.s.tt - 1) / g.s.tt), (unsigned)g.s.py);
   if (p->r.dtype == HMA_BF16) {
-    if (f8)
-      hipLaunchKernelGGL((rope_fwd_kernel<Bf16, true, true>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
-    else
-      hipLaunchKernelGGL((rope_fwd_kernel<Bf16, true, false>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
+    if (f8) launch_fwd<Bf16, true, true>((hipStream_t)stream, g);
+    else launch_fwd<Bf16, true, false>((hipStream_t)stream, g);
   } else {
-    if (f8)
-      hipLaunchKernelGGL((rope_fwd_kernel<_Float16, true, true>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
-    else
-      hipLaunchKernelGGL((rope_fwd_kernel<_Float16, true, false>), grid, dim3(TPB), 0, (hipStream_t)stream, g);
+    if (f8) launch_fwd<_Float16, true, true>((hipStream_t)stream, g);
+    else launch_fwd<_Float16, true, false>((hipStream_t)stream, g);
   }
   HMA_CHECK_LAUNCH();
   return 0;

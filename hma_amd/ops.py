@@ -327,15 +327,24 @@ _NORM = {"none": 0, "rms": 1, "layer": 2}
 _QK_ROPE_WS_GROUPS = 1024
 
 
-def _device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
-    """Every tensor on `first`'s GPU; the context in which its kernels are launched (nothing where that GPU is the current one)."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise RuntimeError("hma ops run on the HIP kernels only (got a %s tensor)" % dev.type)
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+_HERE = contextlib.nullcontext()
+
+
+def _device(*ts: Optional[torch.Tensor]):
+    """Every tensor on the first one's GPU; the context in which its kernels are launched (nothing where that GPU is the current one).
+    These wrappers stand in front of launches of a few microseconds: they look at each tensor once and hold their tests to plain
+    comparisons."""
+    i = ts[0].get_device()
+    if i < 0:
+        raise RuntimeError("hma ops run on the HIP kernels only (got a %s tensor)" % ts[0].device.type)
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            raise ValueError(f"tensors on {ts[0].device} and {t.device}")
+    return _HERE if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _need(ok: bool, what: str) -> None:
@@ -343,11 +352,16 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """(tokens, heads, d) with contiguous 16-byte aligned rows: t itself, or a contiguous copy where its strides are others."""
     s0, s1, s2 = t.stride()
-    m = 16 // t.element_size() - 1
-    return t if s2 == 1 and not ((s0 | s1) & m) and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+    if s2 == 1 and not (s0 | s1) & (3 if t.dtype == F32 else 7) and not t.data_ptr() & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0, trained: int = 8192, slow: float = 1.0,
@@ -392,7 +406,8 @@ def _fill_rope(r, dtype, d: int, tokens: int, freqs, positions, axes, interleave
     if axes is not None and rot:
         _need(axes.dtype == torch.int32 and axes.shape == freqs.shape and axes.is_contiguous(), "axes: int32 (rot / 2,) contiguous")
         r.axes = axes.data_ptr()
-    _need(norm in _NORM, f"norm {norm!r}: none, rms or layer")
+    if norm not in _NORM:
+        raise ValueError(f"norm {norm!r}: none, rms or layer")
     wt = None
     for w in (q_weight, q_bias, k_weight, k_bias):
         if w is not None:
@@ -429,9 +444,9 @@ def qk_rope_fwd(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor],
     p = QkRope()
     with _device(q, k, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias):
         qr, kr = _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
-        qo, ko = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        qo, ko = _like(q), _like(k)
         p.q_out, p.k_out = qo.data_ptr(), ko.data_ptr()
-        _lib.call("hma_qk_rope_fwd", stream_ptr(), C.byref(p))
+        _lib.call("hma_qk_rope_fwd", _stream(q), C.byref(p))
     return qo, ko
 
 
@@ -447,7 +462,7 @@ def qk_rope_bwd(dy_q: torch.Tensor, dy_k: torch.Tensor, q: torch.Tensor, k: torc
         p.dy_q, p.dy_k = gq.data_ptr(), gk.data_ptr()
         p.dyq_tok, p.dyq_head, _ = gq.stride()
         p.dyk_tok, p.dyk_head, _ = gk.stride()
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        dq, dk = _like(q), _like(k)
         dw = [None if w is None else torch.empty_like(w) for w in (q_weight, q_bias, k_weight, k_bias)]
         p.dq, p.dk = dq.data_ptr(), dk.data_ptr()
         p.dq_w, p.dq_b, p.dk_w, p.dk_b = (ptr(w) for w in dw)
@@ -455,7 +470,7 @@ def qk_rope_bwd(dy_q: torch.Tensor, dy_k: torch.Tensor, q: torch.Tensor, k: torc
         if any(w is not None for w in dw):
             ws = torch.empty(_QK_ROPE_WS_GROUPS * 4 * q.shape[2], dtype=F32, device=q.device)
             p.ws, p.ws_floats = ws.data_ptr(), ws.numel()
-        _lib.call("hma_qk_rope_bwd", stream_ptr(), C.byref(p))
+        _lib.call("hma_qk_rope_bwd", _stream(q), C.byref(p))
     return (dq, dk, *dw)
 
 
@@ -508,12 +523,12 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         if q is not None:
             _need(q.dim() == 3 and q.shape[0] == tokens and q.shape[2] == d and q.dtype == k.dtype, "q: (tokens, heads, d) of k's type")
             if q_out is None:
-                q_out, p.zero_tail = torch.empty(q.shape, dtype=q.dtype, device=q.device), 1
+                q_out, p.zero_tail = _like(q), 1
             _need(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous(), "q_out: q's shape and type, contiguous")
             q = _rows16(q)
             p.q, p.q_out, p.hq = q.data_ptr(), q_out.data_ptr(), q.shape[1]
             p.q_tok, p.q_head, _ = q.stride()
-        _lib.call("hma_kv_append", stream_ptr(), C.byref(p))
+        _lib.call("hma_kv_append", _stream(k), C.byref(p))
     return q_out
 
 
@@ -540,7 +555,7 @@ def attn_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         p.q_tok, p.q_head, _ = q.stride()
         _need((out is None) == (lse is None), "out and lse together")
         if out is None:
-            out, lse, p.zero_tail = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(q.shape[:2], dtype=F32, device=q.device), 1
+            out, lse, p.zero_tail = _like(q), q.new_empty(q.shape[:2], dtype=F32), 1
         _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and lse.shape == q.shape[:2] and lse.dtype == F32 and
               lse.is_contiguous(), "out: q's shape and type, lse: fp32 (tokens, heads), contiguous")
         p.q, p.o, p.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
@@ -548,5 +563,5 @@ def attn_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _lib.call("hma_attn_paged_ws", C.byref(p), C.byref(n))
         ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
         p.ws, p.ws_bytes = ptr(ws), n.value
-        _lib.call("hma_attn_paged_fwd", stream_ptr(), C.byref(p))
+        _lib.call("hma_attn_paged_fwd", _stream(q), C.byref(p))
     return out, lse
