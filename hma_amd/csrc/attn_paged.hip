@@ -214,19 +214,24 @@ struct Rows {
       for (int i = 0; i < D / 16; ++i) s[k] = Op<T>::mfma(*reinterpret_cast<const uint4*>(p + k * 32 * (D + PAD) + i * 16), q[i], s[k]);
     }
   }
-  // what a row does not see, and keys without a page (bits of `bad`), out of the scores
+  // what a row does not see out of the scores
   template <int KB>
-  __device__ __forceinline__ void mask(f32x16_t (&s)[KB], int key0, uint64_t bad) const {
-    const int half = (threadIdx.x & 63) >> 5;
-    const uint32_t span = (uint32_t)max(hi - lo, 0);
+  __device__ __forceinline__ void mask(f32x16_t (&s)[KB], int key0) const {
+    const uint32_t first = (uint32_t)(key0 - lo + 4 * ((threadIdx.x & 63) >> 5)), span = (uint32_t)max(hi - lo, 0);
 #pragma unroll
     for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i = k * 32 + 8 * (e >> 2) + 4 * half + (e & 3);
-        const bool seen = (uint32_t)(key0 + i - lo) < span && !((bad >> i) & 1);
-        s[k][e] = seen ? s[k][e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) s[k][e] = first + (k * 32 + 8 * (e >> 2) + (e & 3)) < span ? s[k][e] : -INFINITY;
+  }
+  // keys without a page (bits of `bad`) out of the scores
+  template <int KB>
+  __device__ __forceinline__ void mask_bad(f32x16_t (&s)[KB], uint64_t bad) const {
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const uint32_t w = (uint32_t)(bad >> (k * 32)) >> (4 * ((threadIdx.x & 63) >> 5));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[k][e] = w & (1u << (8 * (e >> 2) + (e & 3))) ? -INFINITY : s[k][e];
+    }
   }
   // s -> probabilities relative to the running maximum, packed as the second product's operand; c: the scores' factor in powers of two
   template <int KB>
@@ -326,50 +331,73 @@ struct Rows {
 };
 
 // ------------------------------------------------------------------------------------- loads of a block of keys
-// A group of THREADS threads loads KEYS rows of 16-byte pieces; lane l of each wave knows the page and the place in it of key l.
-template <typename T, int D, bool F8, int KEYS, int THREADS>
+// THREADS threads load KEYS rows of 16-byte pieces, a wave RPW rows an instruction; lane l of each wave knows the page and the place in it
+// of key l.  ALIGNED: the page size is a multiple of RPW, so the rows of an instruction lie in one page one behind the other and their
+// address is scalar but for the lane's piece; otherwise each lane fetches its row's page by a lane exchange and multiplies by itself.
+template <typename T, int D, bool F8, int KEYS, int THREADS, bool ALIGNED>
 struct Loader {
-  static constexpr int BYTES = F8 ? D : 2 * D, CPR = BYTES / 16, RPI = THREADS / CPR, NI = RPI < KEYS ? KEYS / RPI : 1;
-  static_assert((KEYS % RPI == 0 || RPI == 2 * KEYS) && KEYS <= 64, "");  // 32-byte rows: 128 of the 256 threads load 64
+  static constexpr int BYTES = F8 ? D : 2 * D, CPR = BYTES / 16, RPW = 64 / CPR, RPI = THREADS / CPR, NI = RPI < KEYS ? KEYS / RPI : 1;
+  static_assert((KEYS % RPI == 0 || RPI % KEYS == 0) && KEYS <= 64, "");  // short rows: threads with nothing to load repeat what others do
 
-  static __device__ __forceinline__ void load(const uint8_t* c, int64_t page, int64_t tok, int pg, int off, int tid, uint4 (&r)[NI]) {
+  // tid = wave * 64 + lane
+  static __device__ __forceinline__ void load(const uint8_t* c, int64_t page, int64_t tok, int pg, int off, int wave, int lane, uint4 (&r)[NI]) {
+    if (ALIGNED) {
+      const uint32_t mine = (uint32_t)(lane / CPR) * (uint32_t)tok + (lane % CPR) * 16;  // below 2^31: the host's check
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int row = (i * RPI + tid / CPR) % KEYS;
-      const int p = __shfl(pg, row, 64), f = __shfl(off, row, 64);
-      r[i] = *reinterpret_cast<const uint4*>(c + (p < 0 ? 0 : p * page + f * tok) + (tid % CPR) * 16);
+      for (int i = 0; i < NI; ++i) {
+        const int row = (i * RPI + wave * RPW) % KEYS;
+        const int p = __builtin_amdgcn_readlane(pg, row), f = __builtin_amdgcn_readlane(off, row);
+        r[i] = *reinterpret_cast<const uint4*>(c + (p < 0 ? 0 : p * page + f * tok) + mine);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = (i * RPI + wave * RPW + lane / CPR) % KEYS;
+        const int p = __shfl(pg, row, 64), f = __shfl(off, row, 64);
+        r[i] = *reinterpret_cast<const uint4*>(c + (p < 0 ? 0 : p * page + f * tok) + (lane % CPR) * 16);
+      }
     }
   }
-  // `gaps`: some key has no page (pg < 0): zeros
-  static __device__ __forceinline__ void store(uint16_t* t, int pg, bool gaps, int tid, uint4 (&r)[NI]) {
+  // `gaps`: some key is not seen or has no page (`ok` false for lane = key): zeros
+  static __device__ __forceinline__ void store(uint16_t* t, bool ok, bool gaps, int wave, int lane, uint4 (&r)[NI]) {
+    if (gaps) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const bool have = __shfl((int)ok, (i * RPI + wave * RPW + lane / CPR) % KEYS, 64);
+        r[i].x = have ? r[i].x : 0u; r[i].y = have ? r[i].y : 0u; r[i].z = have ? r[i].z : 0u; r[i].w = have ? r[i].w : 0u;
+      }
+    }
+    uint16_t* p = t + ((wave * RPW + lane / CPR) % KEYS) * (D + PAD) + (lane % CPR) * (F8 ? 16 : 8);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int row = (i * RPI + tid / CPR) % KEYS;  // more threads than pieces: the second half repeats the first's
-      if (gaps && __shfl(pg, row, 64) < 0) r[i] = make_uint4(0, 0, 0, 0);
-      uint16_t* p = t + row * (D + PAD) + (tid % CPR) * (F8 ? 16 : 8);
+      uint16_t* w = p + i * RPI * (D + PAD);
       if (F8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(Op<T>::widen(r[i].x, false), Op<T>::widen(r[i].x, true), Op<T>::widen(r[i].y, false), Op<T>::widen(r[i].y, true));
-        *reinterpret_cast<uint4*>(p + 8) = make_uint4(Op<T>::widen(r[i].z, false), Op<T>::widen(r[i].z, true), Op<T>::widen(r[i].w, false), Op<T>::widen(r[i].w, true));
+        *reinterpret_cast<uint4*>(w) = make_uint4(Op<T>::widen(r[i].x, false), Op<T>::widen(r[i].x, true), Op<T>::widen(r[i].y, false), Op<T>::widen(r[i].y, true));
+        *reinterpret_cast<uint4*>(w + 8) = make_uint4(Op<T>::widen(r[i].z, false), Op<T>::widen(r[i].z, true), Op<T>::widen(r[i].w, false), Op<T>::widen(r[i].w, true));
       } else {
-        *reinterpret_cast<uint4*>(p) = r[i];
+        *reinterpret_cast<uint4*>(w) = r[i];
       }
     }
   }
 };
 
-// The page of key `key` of a sequence, -1 where the tile does not see it; `lost`: seen, but its page is none of the cache's
+// The page of key `key` of a sequence and its place there.  `seen`: by some row of the tile and in a page of the cache; `lost`: seen, but
+// its page is none.  Of a key outside what the tile sees the page is looked up too where the table has one: in a block that is seen in
+// part the rows of one load go by the page of its first.
 struct Place {
   int32_t pg, off;
-  bool lost;
+  bool seen, lost;
 };
-__device__ __forceinline__ Place find_page(const Args& a, const int32_t* table, int key, const Tile& t) {
-  Place p = {-1, 0, false};
-  if (key >= t.lo_min && key < t.hi_max) {
+__device__ __forceinline__ Place find_page(const Args& a, const int32_t* table, int key, int kv, const Tile& t) {
+  Place p = {-1, 0, false, false};
+  if (key >= 0 && key < kv) {
     const int32_t i = (int32_t)(((uint64_t)(uint32_t)key * a.page_mul) >> (31 + a.page_shift));
     p.off = key - i * a.page;
     const int32_t pg = table[i];
-    p.lost = pg < 0 || pg >= a.pages;
-    p.pg = p.lost ? -1 : pg;
+    const bool in = key >= t.lo_min && key < t.hi_max, good = pg >= 0 && pg < a.pages;
+    p.pg = good ? pg : -1;
+    p.seen = in && good;
+    p.lost = in && !good;
   }
   return p;
 }
@@ -393,10 +421,10 @@ __device__ __forceinline__ int share_of(int groups) {
 }
 
 // ------------------------------------------------------------------------------------- few rows: the waves take different keys
-template <typename T, int D, bool F8, int KB>
+template <typename T, int D, bool F8, int KB, bool ALIGNED>
 __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
   constexpr int TR = 32, KEYS = 32 * KB, TK = WAVES * KEYS, LD = D + PAD, NO = D / 32;
-  typedef Loader<T, D, F8, KEYS, 64> Ld;
+  typedef Loader<T, D, F8, KEYS, 64, ALIGNED> Ld;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int64_t wsum[WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -440,29 +468,30 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
     while (je > j && (int64_t)t.start + (int64_t)(je - 1) * TK + wave * KEYS >= t.hi_max) --je;
     if (j < je) {
       const int kl = lane & (KEYS - 1);
-      Place now = find_page(a, table, key_of(j) + kl, t), next = now;
+      Place now = find_page(a, table, key_of(j) + kl, s.kv, t), next = now;
       uint4 kr[Ld::NI], vr[Ld::NI];
-      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, lane, kr);
-      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, lane, vr);
-      if (j + 1 < je) next = find_page(a, table, key_of(j + 1) + kl, t);
+      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, 0, lane, kr);
+      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, 0, lane, vr);
+      if (j + 1 < je) next = find_page(a, table, key_of(j + 1) + kl, s.kv, t);
       for (; j < je; ++j) {
         const int key0 = key_of(j);
-        const bool gaps = __ballot(now.pg < 0) != 0, more = j + 1 < je;
+        const bool gaps = __ballot(!now.seen) != 0, more = j + 1 < je;
         const uint64_t bad = __ballot(now.lost);
         f32x16_t sc[KB];
         uint4 p[KB][2];
-        Ld::store(mine, now.pg, gaps, lane, kr);
-        if (more) Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, lane, kr);
+        Ld::store(mine, now.seen, gaps, 0, lane, kr);
+        if (more) Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, 0, lane, kr);
         wave_lds_order();
         r.template scores<KB>(mine, sc);
-        if (bad || key0 < t.lo_max || key0 + KEYS > t.hi_min) r.template mask<KB>(sc, key0, bad);
+        if (key0 < t.lo_max || key0 + KEYS > t.hi_min) r.template mask<KB>(sc, key0);
+        if (bad) r.template mask_bad<KB>(sc, bad);
         r.template softmax<KB>(sc, c, p);
         wave_lds_order();
-        Ld::store(mine, now.pg, gaps, lane, vr);
+        Ld::store(mine, now.seen, gaps, 0, lane, vr);
         if (more) {
-          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, lane, vr);
+          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, 0, lane, vr);
           now = next;
-          if (j + 2 < je) next = find_page(a, table, key_of(j + 2) + kl, t);
+          if (j + 2 < je) next = find_page(a, table, key_of(j + 2) + kl, s.kv, t);
         }
         wave_lds_order();
         r.template values<KB>(mine, p);
@@ -506,10 +535,10 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 128
-template <typename T, int D, bool F8, bool SPLIT>
+template <typename T, int D, bool F8, bool SPLIT, bool ALIGNED>
 __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
   constexpr int TR = 128, TK = 64, LD = D + PAD, BUF = 2 * TK * LD;
-  typedef Loader<T, D, F8, TK, TPB> Ld;
+  typedef Loader<T, D, F8, TK, TPB, ALIGNED> Ld;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int64_t wsum[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -578,22 +607,22 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
     const int je = min(j1, max((t.hi_max - t.start + TK - 1) / TK, 0));
     int j = j0;
     if (j < je) {
-      Place now = find_page(a, table, t.start + j * TK + lane, t), next = now;
+      Place now = find_page(a, table, t.start + j * TK + lane, s.kv, t), next = now;
       uint4 kr[Ld::NI], vr[Ld::NI];
-      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, tid, kr);
-      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, tid, vr);
-      if (j + 1 < je) next = find_page(a, table, t.start + (j + 1) * TK + lane, t);
+      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, wave, lane, kr);
+      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, wave, lane, vr);
+      if (j + 1 < je) next = find_page(a, table, t.start + (j + 1) * TK + lane, s.kv, t);
       for (int buf = 0; j < je; ++j, buf ^= 1) {
         uint16_t *kt = tiles + buf * BUF, *vt = kt + TK * LD;
-        const bool gaps = __ballot(now.pg < 0) != 0;
+        const bool gaps = __ballot(!now.seen) != 0;
         const uint64_t bad = __ballot(now.lost);
-        Ld::store(kt, now.pg, gaps, tid, kr);
-        Ld::store(vt, now.pg, gaps, tid, vr);
+        Ld::store(kt, now.seen, gaps, wave, lane, kr);
+        Ld::store(vt, now.seen, gaps, wave, lane, vr);
         if (j + 1 < je) {
-          Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, tid, kr);
-          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, tid, vr);
+          Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, wave, lane, kr);
+          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, wave, lane, vr);
           now = next;
-          if (j + 2 < je) next = find_page(a, table, t.start + (j + 2) * TK + lane, t);
+          if (j + 2 < je) next = find_page(a, table, t.start + (j + 2) * TK + lane, s.kv, t);
         }
         __syncthreads();  // one barrier a tile: the other buffer's readers passed the last one
         const int key0 = t.start + j * TK;
@@ -601,7 +630,8 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
           f32x16_t sc[2];
           uint4 p[2][2];
           r.template scores<2>(kt, sc);
-          if (bad || key0 < w.lo_max || key0 + TK > w.hi_min) r.template mask<2>(sc, key0, bad);
+          if (key0 < w.lo_max || key0 + TK > w.hi_min) r.template mask<2>(sc, key0);
+          if (bad) r.template mask_bad<2>(sc, bad);
           r.template softmax<2>(sc, c, p);
           r.template values<2>(vt, p);
         }
@@ -699,7 +729,9 @@ Plan plan_of(const hma_attn_paged_t* p) {
   // no more workgroups than units: row tiles x key tiles of the longest sequence that the table can hold
   const int64_t most = ((int64_t)p->table_w * p->page + r.tk - 1) / r.tk;
   const int64_t units = r.slots * p->hk * (most > 0 ? most : 1);
-  r.groups = (int)(units < 2 * CUS ? (units > 0 ? units : 1) : 2 * CUS);
+  // as many workgroups as are resident together (their registers and LDS), each with one share
+  const int64_t room = CUS * (r.few ? (p->d == 32 ? 3 : 2) : (p->d == 128 ? 2 : p->d == 64 ? 3 : 4));
+  r.groups = (int)(units < room ? (units > 0 ? units : 1) : room);
   r.ws = r.split ? (int64_t)r.groups * 2 * r.tr * (p->d + 2) * 4 + (p->seqs + 2) * 8 : 0;
   return r;
 }
@@ -718,22 +750,22 @@ int allow_lds() {
   return 0;
 }
 
-template <typename T, int D, bool F8>
+template <typename T, int D, bool F8, bool ALIGNED>
 int launch(hipStream_t st, const Args& a, const Plan& r) {
   constexpr int KB = D == 128 && !F8 ? 1 : 2, LD = D + PAD;
   const size_t units = (size_t)(a.seqs + 1) * 8;
   if (r.few) {
     const size_t lds = (size_t)WAVES * 32 * KB * LD * 2 + units;
-    if (const int rc = allow_lds<attn_few_kernel<T, D, F8, KB>>()) return rc;
-    hipLaunchKernelGGL((attn_few_kernel<T, D, F8, KB>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
+    if (const int rc = allow_lds<attn_few_kernel<T, D, F8, KB, ALIGNED>>()) return rc;
+    hipLaunchKernelGGL((attn_few_kernel<T, D, F8, KB, ALIGNED>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
   } else {
     const size_t lds = (size_t)2 * 2 * 64 * LD * 2 + (r.split ? units : 0);
     if (r.split) {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, true>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, true>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, true, ALIGNED>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, true, ALIGNED>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
     } else {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, false>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, false>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), lds, st, a);
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, false, ALIGNED>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, false, ALIGNED>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), lds, st, a);
     }
   }
   HMA_CHECK_LAUNCH();
@@ -744,9 +776,15 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
   }
   return 0;
 }
+template <typename T, int D, bool F8>
+int launch_a(hipStream_t st, const Args& a, const Plan& r) {
+  constexpr int RPW = 64 / ((F8 ? D : 2 * D) / 16);  // rows of a wave's load (Loader)
+  const bool fits = a.kc_tok * RPW < 0x40000000 && a.vc_tok * RPW < 0x40000000;
+  return a.page % RPW == 0 && fits ? launch<T, D, F8, true>(st, a, r) : launch<T, D, F8, false>(st, a, r);
+}
 template <typename T, int D>
 int launch_f8(hipStream_t st, const Args& a, const Plan& r, bool e) {
-  return e ? launch<T, D, true>(st, a, r) : launch<T, D, false>(st, a, r);
+  return e ? launch_a<T, D, true>(st, a, r) : launch_a<T, D, false>(st, a, r);
 }
 template <typename T>
 int launch_d(hipStream_t st, const Args& a, const Plan& r, bool e, int d) {
