@@ -37,7 +37,7 @@ typedef short v8s16_t __attribute__((ext_vector_type(8)));
 constexpr int TPB = 256, WAVES = 4;
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
 constexpr float LAZY = 8.0f;  // how far (in powers of two) a row may exceed its running maximum before O is rescaled
-constexpr int PAD = 16;       // LDS rows of D + 16 values: the 4 rows of a transposing read and the 8 rows of a 16-byte read hit 64 banks once
+constexpr int PAD = 16;       // few rows: LDS rows of D + 16 values (two-way conflicts of the transposing reads, which do not bound that kernel)
 
 struct Args {
   const void* q;
@@ -107,11 +107,12 @@ __device__ __forceinline__ int key_tiles(const Args& a, const Seq& s, int tr, in
   return max(t, 1);
 }
 // base[b] = units before sequence b, by the whole workgroup
+template <int NW>
 __device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t* wsum, int tr, int tk) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t carry = 0;
   if (threadIdx.x == 0) base[0] = 0;
-  for (int b0 = 0; b0 < a.seqs; b0 += TPB) {
+  for (int b0 = 0; b0 < a.seqs; b0 += 64 * NW) {
     const int b = b0 + threadIdx.x;
     int64_t v = 0;
     if (b < a.seqs) {
@@ -126,7 +127,7 @@ __device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t
     if (lane == 63) wsum[wave] = v;
     __syncthreads();
     int64_t before = carry;
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < NW; ++w) {
       if (w < wave) before += wsum[w];
       carry += wsum[w];
     }
@@ -201,6 +202,11 @@ struct Rows {
     l = 0.f;
   }
 
+  // the rows' loads waited for here (the compiler, which does not count LDS DMA, would wait for them -- and for all in flight -- in the loop)
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
+  }
   // scores of KB blocks of 32 keys; kt: their rows in LDS
   template <int KB>
   __device__ __forceinline__ void scores(const uint16_t* kt, f32x16_t (&s)[KB]) const {
@@ -233,9 +239,9 @@ struct Rows {
       for (int e = 0; e < 16; ++e) s[k][e] = w & (1u << (8 * (e >> 2) + (e & 3))) ? -INFINITY : s[k][e];
     }
   }
-  // s -> probabilities relative to the running maximum, packed as the second product's operand; c: the scores' factor in powers of two
+  // the largest score of a row's KB blocks in powers of two (c: the scores' factor)
   template <int KB>
-  __device__ __forceinline__ void softmax(f32x16_t (&s)[KB], float c, uint4 (&p)[KB][2]) {
+  __device__ __forceinline__ float largest(const f32x16_t (&s)[KB], float c) const {
     float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
     for (int k = 0; k < KB; ++k)
@@ -244,8 +250,12 @@ struct Rows {
         x0 = __builtin_fmaxf(__builtin_fmaxf(x0, s[k][e]), s[k][e + 1]);
         x1 = __builtin_fmaxf(__builtin_fmaxf(x1, s[k][e + 2]), s[k][e + 3]);
       }
-    float x = fmaxf(x0, x1);
-    x = fmaxf(x, __shfl_xor(x, 32, 64)) * c;
+    const uint32_t x = __float_as_uint(fmaxf(x0, x1));
+    const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);  // the two half-waves' values in every lane
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
+  }
+  // the running maximum raised where a row exceeds it by far
+  __device__ __forceinline__ void raise(float x) {
     if (__ballot(x > m + LAZY)) {  // also where m is still -inf
       const float up = fmaxf(m, x), f = m == -INFINITY ? 0.f : fast_exp2(m - up);
       l *= f;
@@ -255,22 +265,22 @@ struct Rows {
         for (int e = 0; e < 16; ++e) o[i][e] *= f;
       m = up;
     }
+  }
+  // a block of scores -> probabilities relative to the running maximum, packed as the second product's operand, and their sum
+  __device__ __forceinline__ void weigh(f32x16_t& s, float c, uint4 (&p)[2]) {
     const float sub = m == -INFINITY ? 0.f : m;
     float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-    for (int k = 0; k < KB; ++k) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        s[k][e] = fast_exp2(__builtin_fmaf(s[k][e], c, -sub));
-        s[k][e + 1] = fast_exp2(__builtin_fmaf(s[k][e + 1], c, -sub));
-        l0 += s[k][e];
-        l1 += s[k][e + 1];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        p[k][h] = make_uint4(Op<T>::pack(s[k][8 * h], s[k][8 * h + 1]), Op<T>::pack(s[k][8 * h + 2], s[k][8 * h + 3]),
-                             Op<T>::pack(s[k][8 * h + 4], s[k][8 * h + 5]), Op<T>::pack(s[k][8 * h + 6], s[k][8 * h + 7]));
+    for (int e = 0; e < 16; e += 2) {
+      s[e] = fast_exp2(__builtin_fmaf(s[e], c, -sub));
+      s[e + 1] = fast_exp2(__builtin_fmaf(s[e + 1], c, -sub));
+      l0 += s[e];
+      l1 += s[e + 1];
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      p[h] = make_uint4(Op<T>::pack(s[8 * h], s[8 * h + 1]), Op<T>::pack(s[8 * h + 2], s[8 * h + 3]), Op<T>::pack(s[8 * h + 4], s[8 * h + 5]),
+                        Op<T>::pack(s[8 * h + 6], s[8 * h + 7]));
     l += l0 + l1;
   }
   // o += V^T p; vt: the values' rows in LDS.  The transposing read gives lane (d = l & 31, half) the rows 4 half + {0..3} and those + 8 of
@@ -381,26 +391,23 @@ struct Loader {
   }
 };
 
-// The page of key `key` of a sequence and its place there.  `seen`: by some row of the tile and in a page of the cache; `lost`: seen, but
-// its page is none.  Of a key outside what the tile sees the page is looked up too where the table has one: in a block that is seen in
-// part the rows of one load go by the page of its first.
+// The page of key `key` of a sequence and its place there.  look() only issues the table's load (a key behind the sequence: its last
+// page, row 0); what is asked of the page number waits for it, so it is asked a tile later.
 struct Place {
-  int32_t pg, off;
-  bool seen, lost;
-};
-__device__ __forceinline__ Place find_page(const Args& a, const int32_t* table, int key, int kv, const Tile& t) {
-  Place p = {-1, 0, false, false};
-  if (key >= 0 && key < kv) {
-    const int32_t i = (int32_t)(((uint64_t)(uint32_t)key * a.page_mul) >> (31 + a.page_shift));
-    p.off = key - i * a.page;
-    const int32_t pg = table[i];
-    const bool in = key >= t.lo_min && key < t.hi_max, good = pg >= 0 && pg < a.pages;
-    p.pg = good ? pg : -1;
-    p.seen = in && good;
-    p.lost = in && !good;
+  int32_t raw, off, key;
+  __device__ __forceinline__ void look(const Args& a, const int32_t* table, int k, int kv) {  // kv > 0
+    const int32_t i = (int32_t)(((uint64_t)(uint32_t)min(k, kv - 1) * a.page_mul) >> (31 + a.page_shift));
+    key = k;
+    off = k < kv ? k - i * a.page : 0;
+    raw = table[i];
   }
-  return p;
-}
+  __device__ __forceinline__ bool good(const Args& a) const { return (uint32_t)raw < (uint32_t)a.pages; }
+  __device__ __forceinline__ bool in(const Tile& t) const { return key >= t.lo_min && key < t.hi_max; }
+  __device__ __forceinline__ bool seen(const Args& a, const Tile& t) const { return in(t) && good(a); }   // by some row of the tile, and in the cache
+  __device__ __forceinline__ bool lost(const Args& a, const Tile& t) const { return in(t) && !good(a); }  // its page is none of the cache's
+  // bytes from the head's first row to key's row
+  __device__ __forceinline__ int64_t at(const Args& a, int64_t page, int64_t tok) const { return good(a) ? raw * page + off * tok : 0; }
+};
 
 // rows behind the last sequence
 template <int D>
@@ -408,7 +415,7 @@ __device__ __forceinline__ void clear_tail(const Args& a) {
   if (!a.zero_tail) return;
   const int64_t end = min(max((int64_t)a.cu[a.seqs], (int64_t)0), a.tokens);
   const int64_t rows = (a.tokens - end) * a.hq, n = rows * (D / 8), at = end * a.hq;
-  for (int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x; i < n; i += (int64_t)gridDim.x * TPB) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     *reinterpret_cast<uint4*>((uint16_t*)a.o + at * D + i * 8) = make_uint4(0, 0, 0, 0);
     if (a.lse && i % (D / 8) == 0) a.lse[at + i / (D / 8)] = -INFINITY;
   }
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
   int64_t* base = (int64_t*)(smem + WAVES * KEYS * LD * 2);
   clear_tail<D>(a);
   if (a.seqs == 0) return;
-  unit_table(a, base, wsum, TR, TK);
+  unit_table<WAVES>(a, base, wsum, TR, TK);
   const int64_t total = base[a.seqs], each = (total + a.groups - 1) / a.groups;
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i <= a.seqs; i += TPB) a.units[i] = base[i];
@@ -468,30 +475,36 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
     while (je > j && (int64_t)t.start + (int64_t)(je - 1) * TK + wave * KEYS >= t.hi_max) --je;
     if (j < je) {
       const int kl = lane & (KEYS - 1);
-      Place now = find_page(a, table, key_of(j) + kl, s.kv, t), next = now;
+      Place now, next;
+      now.look(a, table, key_of(j) + kl, s.kv);
+      next = now;
+      int pg = now.good(a) ? now.raw : -1;
       uint4 kr[Ld::NI], vr[Ld::NI];
-      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, 0, lane, kr);
-      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, 0, lane, vr);
-      if (j + 1 < je) next = find_page(a, table, key_of(j + 1) + kl, s.kv, t);
+      Ld::load(kc, a.kc_page, a.kc_tok, pg, now.off, 0, lane, kr);
+      Ld::load(vc, a.vc_page, a.vc_tok, pg, now.off, 0, lane, vr);
+      if (j + 1 < je) next.look(a, table, key_of(j + 1) + kl, s.kv);
       for (; j < je; ++j) {
         const int key0 = key_of(j);
-        const bool gaps = __ballot(!now.seen) != 0, more = j + 1 < je;
-        const uint64_t bad = __ballot(now.lost);
+        const bool seen = now.seen(a, t), gaps = __ballot(!seen) != 0, more = j + 1 < je;
+        const uint64_t bad = __ballot(now.lost(a, t));
         f32x16_t sc[KB];
         uint4 p[KB][2];
-        Ld::store(mine, now.seen, gaps, 0, lane, kr);
-        if (more) Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, 0, lane, kr);
+        Ld::store(mine, seen, gaps, 0, lane, kr);
+        pg = next.good(a) ? next.raw : -1;
+        if (more) Ld::load(kc, a.kc_page, a.kc_tok, pg, next.off, 0, lane, kr);
         wave_lds_order();
         r.template scores<KB>(mine, sc);
         if (key0 < t.lo_max || key0 + KEYS > t.hi_min) r.template mask<KB>(sc, key0);
         if (bad) r.template mask_bad<KB>(sc, bad);
-        r.template softmax<KB>(sc, c, p);
+        r.raise(r.template largest<KB>(sc, c));
+#pragma unroll
+        for (int k = 0; k < KB; ++k) r.weigh(sc[k], c, p[k]);
         wave_lds_order();
-        Ld::store(mine, now.seen, gaps, 0, lane, vr);
+        Ld::store(mine, seen, gaps, 0, lane, vr);
         if (more) {
-          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, 0, lane, vr);
+          Ld::load(vc, a.vc_page, a.vc_tok, pg, next.off, 0, lane, vr);
           now = next;
-          if (j + 2 < je) next = find_page(a, table, key_of(j + 2) + kl, s.kv, t);
+          if (j + 2 < je) next.look(a, table, key_of(j + 2) + kl, s.kv);
         }
         wave_lds_order();
         r.template values<KB>(mine, p);
@@ -534,25 +547,43 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
   }
 }
 
-// ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 128
-template <typename T, int D, bool F8, bool SPLIT, bool ALIGNED>
-__global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
-  constexpr int TR = 128, TK = 64, LD = D + PAD, BUF = 2 * TK * LD;
-  typedef Loader<T, D, F8, TK, TPB, ALIGNED> Ld;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  __shared__ int64_t wsum[WAVES];
+// ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 32 NW
+// The NW waves share tiles of 64 keys and values, two of each in LDS.  A wave has two companions at most on its SIMD and issues an
+// instruction every five cycles or so, whatever its kind, so the instructions around the products and the exponentials are what there is
+// to save: 16-bit tiles come by LDS DMA in pieces of 1 KB, whose addresses are scalar (two lane reads and two additions a piece) plus one
+// register of lane offsets; a tile of keys is 16 such pieces at D = 128, two a wave.
+// Layout of a tile: piece = 64 / CPR rows (CPR = D / 8 chunks of 16 bytes each), pieces 16 bytes further apart than their size, chunk c of
+// row r at place c ^ turn(r) of its row.  A 16-byte read of 16 rows and a transposing read of 4 rows x 64 bytes then touch every bank once.
+template <int D>
+struct Lay {
+  static constexpr int CPR = D / 8, RPP = 64 / CPR, PIECE = 1024 + (D == 32 ? 0 : 16), PIECES = 64 / RPP, TILE = PIECES * PIECE;
+  static __device__ __forceinline__ int turn(int r) { return D == 128 ? 4 * (r & 3) : D == 64 ? 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1) : (r >> 2) & 3; }
+  static __device__ __forceinline__ int at(int r, int c) { return r / RPP * PIECE + r % RPP * (2 * D) + (c ^ turn(r)) * 16; }
+};
+template <int D, int NW> struct ManyWaves { static constexpr int value = D == 128 ? 2 : D == 64 ? 3 : 4; };  // waves a SIMD
+
+template <typename T, int D, bool F8, int NW, bool ALIGNED>
+__global__ __launch_bounds__(64 * NW, (ManyWaves<D, NW>::value)) void attn_many_kernel(const Args a, const int split) {
+  typedef Lay<D> Y;
+  constexpr int TR = 32 * NW, TK = 64, BUF = 2 * Y::TILE, NO = D / 32;
+  constexpr bool DMA = !F8 && ALIGNED;
+  constexpr int NP = Y::PIECES / NW;  // pieces of a tile per wave
+  static_assert(Y::PIECES % NW == 0, "");
+  // through registers: 16-byte pieces of the cache's rows, NI a thread
+  constexpr int BYTES = F8 ? D : 2 * D, CPR = BYTES / 16, RPW = 64 / CPR, RPI = NW * RPW, NI = RPI < TK ? TK / RPI : 1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [2][keys | values]
+  __shared__ int64_t wsum[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint16_t* tiles = (uint16_t*)smem;  // [2][keys | values][TK][LD]
-  int64_t* base = (int64_t*)(smem + 2 * BUF * 2);
+  int64_t* base = (int64_t*)(smem + 2 * BUF);
   clear_tail<D>(a);
   if (a.seqs == 0) return;
   int64_t u0 = 0, u1 = 1, g = 0;
   int b = 0, slot_qt = 0;
-  if (SPLIT) {
-    unit_table(a, base, wsum, TR, TK);
+  if (split) {
+    unit_table<NW>(a, base, wsum, TR, TK);
     const int64_t total = base[a.seqs], each = (total + a.groups - 1) / a.groups;
     if (blockIdx.x == 0) {
-      for (int i = tid; i <= a.seqs; i += TPB) a.units[i] = base[i];
+      for (int i = tid; i <= a.seqs; i += 64 * NW) a.units[i] = base[i];
       if (tid == 0) a.units[a.seqs + 1] = each;
     }
     g = share_of(a.groups);
@@ -569,15 +600,29 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
     if (b >= a.seqs) return;
     slot_qt = (int)(slot - first_slot(a, b, TR));
   }
+  // lane constants: where this lane's operands lie in a tile
+  const int half = lane >> 5, i16 = lane & 15, g16 = lane >> 4;
+  constexpr int NKA = D == 128 ? 4 : D / 16;
+  uint32_t ka[NKA], va[NO], va8 = 0;
+#pragma unroll
+  for (int s = 0; s < NKA; ++s) ka[s] = Y::at(lane & 31, (D == 128 ? 4 : 2) * s + half);
+#pragma unroll
+  for (int i = 0; i < NO; ++i) va[i] = Y::at(4 * (g16 >> 1) + (i16 >> 2), 4 * i + 2 * (g16 & 1) + ((i16 & 3) >> 1)) + 8 * (i16 & 1);
+  if (D == 32) va8 = Y::at(8 + 4 * (g16 >> 1) + (i16 >> 2), 2 * (g16 & 1) + ((i16 & 3) >> 1)) + 8 * (i16 & 1);
+  const int turned = ((lane % Y::CPR) ^ Y::turn(lane / Y::CPR)) * 16;  // DMA: the chunk that belongs in this lane's place
+  const uint32_t k_off = lane / Y::CPR * (uint32_t)a.kc_tok + turned, v_off = lane / Y::CPR * (uint32_t)a.vc_tok + turned;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(HMA_LDS(uint8_t)*)smem;
+  const bool alike = a.kc_page == a.vc_page && a.kc_tok == a.vc_tok;
+
   for (int64_t u = u0; u < u1;) {
-    if (SPLIT)
+    if (split)
       while (base[b + 1] <= u) ++b;
     const Seq s = seq_of(a, b);
     const int nq = row_tiles(a, s, TR);
     int nt, j0, j1, hk, qt;
     int64_t first = 0;
     Tile t;
-    if (SPLIT) {
+    if (split) {
       nt = key_tiles(a, s, TR, TK);
       const int64_t local = u - base[b], item = local / nt;
       first = u - (local - item * nt);
@@ -600,49 +645,202 @@ __global__ __launch_bounds__(TPB, 2) void attn_many_kernel(const Args a) {
     Rows<T, D> r;
     r.begin(a, s, hk, qt * TR + wave * 32 + (lane & 31));
     // what this wave's 32 rows see (rows that are none see nothing)
-    const int w0 = qt * TR + wave * 32;
-    const bool any = w0 < (int64_t)s.n * a.group;
+    const bool any = qt * TR + wave * 32 < (int64_t)s.n * a.group;
     Tile w = t;
-    if (any) w = tile_of(a, s, qt * WAVES + wave, 32, TK);
+    if (any) w = tile_of(a, s, qt * NW + wave, 32, TK);
     const int je = min(j1, max((t.hi_max - t.start + TK - 1) / TK, 0));
-    int j = j0;
-    if (j < je) {
-      Place now = find_page(a, table, t.start + j * TK + lane, s.kv, t), next = now;
-      uint4 kr[Ld::NI], vr[Ld::NI];
-      Ld::load(kc, a.kc_page, a.kc_tok, now.pg, now.off, wave, lane, kr);
-      Ld::load(vc, a.vc_page, a.vc_tok, now.pg, now.off, wave, lane, vr);
-      if (j + 1 < je) next = find_page(a, table, t.start + (j + 1) * TK + lane, s.kv, t);
-      for (int buf = 0; j < je; ++j, buf ^= 1) {
-        uint16_t *kt = tiles + buf * BUF, *vt = kt + TK * LD;
-        const bool gaps = __ballot(!now.seen) != 0;
-        const uint64_t bad = __ballot(now.lost);
-        Ld::store(kt, now.seen, gaps, wave, lane, kr);
-        Ld::store(vt, now.seen, gaps, wave, lane, vr);
-        if (j + 1 < je) {
-          Ld::load(kc, a.kc_page, a.kc_tok, next.pg, next.off, wave, lane, kr);
-          Ld::load(vc, a.vc_page, a.vc_tok, next.pg, next.off, wave, lane, vr);
-          now = next;
-          if (j + 2 < je) next = find_page(a, table, t.start + (j + 2) * TK + lane, s.kv, t);
+
+    uint4 kr[DMA ? 1 : NI], vr[DMA ? 1 : NI];
+    // tile of `p` on its way: into LDS buffer `buf`, or into registers
+    const auto fetch = [&](const Place& p, int buf) {
+      if (DMA) {
+        const int64_t ko = p.at(a, a.kc_page, a.kc_tok);
+        int64_t vo = ko;
+        if (!alike) vo = p.at(a, a.vc_page, a.vc_tok);
+        const int klo = (int)ko, khi = (int)(ko >> 32), vlo = (int)vo, vhi = (int)(vo >> 32);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int piece = i * NW + wave, row = piece * Y::RPP;
+          const uint32_t to = lds0 + buf * BUF + piece * Y::PIECE;
+          glds16s(kc + (((int64_t)__builtin_amdgcn_readlane(khi, row) << 32) | (uint32_t)__builtin_amdgcn_readlane(klo, row)), k_off, to);
+          glds16s(vc + (((int64_t)__builtin_amdgcn_readlane(vhi, row) << 32) | (uint32_t)__builtin_amdgcn_readlane(vlo, row)), v_off, to + Y::TILE);
         }
-        __syncthreads();  // one barrier a tile: the other buffer's readers passed the last one
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = (i * RPI + wave * RPW + lane / CPR) % TK;
+          const int pg = __shfl(p.good(a) ? p.raw : -1, row, 64), f = __shfl(p.off, row, 64);
+          kr[i] = *reinterpret_cast<const uint4*>(kc + (pg < 0 ? 0 : pg * a.kc_page + f * a.kc_tok) + (lane % CPR) * 16);
+          vr[i] = *reinterpret_cast<const uint4*>(vc + (pg < 0 ? 0 : pg * a.vc_page + f * a.vc_tok) + (lane % CPR) * 16);
+        }
+      }
+    };
+    // the fetched tile into place: values of keys that no row sees are zeros (their scores are masked, but 0 x NaN is a NaN)
+    const auto settle = [&](const Place& p, int buf) {
+      const bool seen = p.seen(a, t), gaps = __ballot(!seen) != 0;
+      uint8_t *kt = smem + buf * BUF, *vt = kt + Y::TILE;
+      if (DMA) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (gaps) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const int piece = i * NW + wave;
+            if (!__shfl((int)seen, piece * Y::RPP + lane / Y::CPR, 64)) *reinterpret_cast<uint4*>(vt + piece * Y::PIECE + lane * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = (i * RPI + wave * RPW + lane / CPR) % TK, ch = lane % CPR;
+          const bool have = !gaps || __shfl((int)seen, row, 64);
+          uint4 v = vr[i];
+          v.x = have ? v.x : 0u; v.y = have ? v.y : 0u; v.z = have ? v.z : 0u; v.w = have ? v.w : 0u;
+          if (F8) {
+            const auto lo = [](const uint4& x) { return make_uint4(Op<T>::widen(x.x, false), Op<T>::widen(x.x, true), Op<T>::widen(x.y, false), Op<T>::widen(x.y, true)); };
+            const auto hi = [](const uint4& x) { return make_uint4(Op<T>::widen(x.z, false), Op<T>::widen(x.z, true), Op<T>::widen(x.w, false), Op<T>::widen(x.w, true)); };
+            *reinterpret_cast<uint4*>(kt + Y::at(row, 2 * ch)) = lo(kr[i]);
+            *reinterpret_cast<uint4*>(kt + Y::at(row, 2 * ch + 1)) = hi(kr[i]);
+            *reinterpret_cast<uint4*>(vt + Y::at(row, 2 * ch)) = lo(v);
+            *reinterpret_cast<uint4*>(vt + Y::at(row, 2 * ch + 1)) = hi(v);
+          } else {
+            *reinterpret_cast<uint4*>(kt + Y::at(row, ch)) = kr[i];
+            *reinterpret_cast<uint4*>(vt + Y::at(row, ch)) = v;
+          }
+        }
+      }
+    };
+    if (j0 < je) {
+      const auto look = [&](Place& p, int j) { p.look(a, table, t.start + j * TK + lane, s.kv); };
+      Place now, next;
+      look(now, j0);
+      look(next, j0 + 1);
+      r.arrive();
+      fetch(now, 0);
+      settle(now, 0);
+      __syncthreads();
+      int buf = 0;
+      for (int j = j0; j < je; ++j, buf ^= 1) {
+        const bool more = j + 1 < je;
+        const uint64_t bad = __ballot(now.lost(a, t));
+        Place after = next;
+        if (more) {
+          fetch(next, buf ^ 1);
+          look(after, j + 2);
+        }
         const int key0 = t.start + j * TK;
         if (any && key0 < w.hi_max && key0 + TK > w.lo_min) {
+          const uint8_t *kt = smem + buf * BUF, *vt = kt + Y::TILE;
+          // Two blocks of 32 keys.  The reads run AHEAD operands in front of the products that use them; the first block's exponentials stand
+          // between the second's products, the second's between the first's values.  The barriers stop the compiler only: left alone it
+          // puts each read right in front of its product and the exponentials behind the last, and the wave waits in both places.
+          constexpr int NS = D / 16, AHEAD = 4;  // operands of a block of 32 keys, of a block of 32 values
+          const auto key_operand = [&](int n) {
+            const int at = D == 128 ? ka[(n % NS) >> 1] + (n & 1) * 32 : ka[n % NS % NKA];
+            return *reinterpret_cast<const uint4*>(kt + at + n / NS * (32 / Y::RPP) * Y::PIECE);
+          };
+          const auto value_operand = [&](int n) {  // 16 keys, 32 columns n % NO
+            const uint8_t* v = vt + n / NO * 16 / Y::RPP * Y::PIECE;
+            const uint8_t* v8 = D == 32 ? v + va8 : v + va[n % NO] + 8 / Y::RPP * Y::PIECE;
+            const v4s16_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HMA_LDS(v4s16_t)*)(v + va[n % NO]));
+            const v4s16_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HMA_LDS(v4s16_t)*)v8);
+            return __builtin_bit_cast(uint4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+          };
+          const bool edge = key0 < w.lo_max || key0 + TK > w.hi_min || bad != 0;
           f32x16_t sc[2];
-          uint4 p[2][2];
-          r.template scores<2>(kt, sc);
-          if (key0 < w.lo_max || key0 + TK > w.hi_min) r.template mask<2>(sc, key0);
-          if (bad) r.template mask_bad<2>(sc, bad);
-          r.template softmax<2>(sc, c, p);
-          r.template values<2>(vt, p);
+          uint4 f[2 * NS], p[2];
+          float sub = r.m == -INFINITY ? 0.f : r.m, sum = 0.f;
+          // probabilities of elements e0 .. e1 - 1 in 32 bits; the scores stay, in case the running maximum turns out too low
+          float x[16];
+          const auto weigh = [&](const f32x16_t& s, int e0, int e1) {
+#pragma unroll
+            for (int e = e0; e < e1; ++e) {
+              x[e] = fast_exp2(__builtin_fmaf(s[e], c, -sub));
+              sum += x[e];
+              if (e & 1) {
+                uint32_t* to = &(&p[e >> 3].x)[(e & 7) >> 1];
+                *to = Op<T>::pack(x[e - 1], x[e]);
+                asm volatile("" : "+v"(*to));
+              }
+            }
+            asm volatile("" : "+v"(sum));  // (here, not where the values are wanted)
+          };
+          // No maximum is sought as long as no row's probabilities of a block add up to more than 16 x 2^LAZY (then none is over that, which
+          // fp16 holds) and every row has a maximum: the sum is needed anyway.  Otherwise: the maximum, and the block again.
+          const auto settle_max = [&](int k) {
+            if (__ballot(!(sum <= 16.0f * 256.0f) || r.m == -INFINITY)) {
+              f32x16_t one[1] = {sc[k]};
+              r.raise(r.template largest<1>(one, c));
+              sub = r.m == -INFINITY ? 0.f : r.m;
+              sum = 0.f;
+              weigh(sc[k], 0, 16);
+            }
+            r.l += sum;
+            sum = 0.f;
+          };
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[0][e] = sc[1][e] = 0.f;
+#pragma unroll
+          for (int n = 0; n < AHEAD; ++n) f[n] = key_operand(n);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            sc[0] = Op<T>::mfma(f[n], r.q[n], sc[0]);
+            if (n + AHEAD < 2 * NS) f[n + AHEAD] = key_operand(n + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (edge) {
+            f32x16_t one[1] = {sc[0]};
+            r.template mask<1>(one, key0);
+            if ((uint32_t)bad) r.template mask_bad<1>(one, (uint32_t)bad);
+            sc[0] = one[0];
+          }
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            sc[1] = Op<T>::mfma(f[n + NS], r.q[n], sc[1]);
+            if (n + NS + AHEAD < 2 * NS) f[n + NS + AHEAD] = key_operand(n + NS + AHEAD);
+            weigh(sc[0], n * 16 / NS, (n + 1) * 16 / NS);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (edge) {
+            f32x16_t one[1] = {sc[1]};
+            r.template mask<1>(one, key0 + 32);
+            if (bad >> 32) r.template mask_bad<1>(one, bad >> 32);
+            sc[1] = one[0];
+          }
+#pragma unroll
+          for (int n = 0; n < AHEAD; ++n) f[n] = value_operand(n);
+          settle_max(0);
+          uint4 p0[2] = {p[0], p[1]};
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            r.o[n % NO] = Op<T>::mfma(f[n], p0[n / NO], r.o[n % NO]);
+            if (n + AHEAD < 2 * NS) f[n + AHEAD] = value_operand(n + AHEAD);
+            weigh(sc[1], n * 16 / NS, (n + 1) * 16 / NS);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          settle_max(1);
+#pragma unroll
+          for (int n = NS; n < 2 * NS; ++n) {
+            r.o[n % NO] = Op<T>::mfma(f[n], p[n % NS / NO], r.o[n % NO]);
+            if (n + AHEAD < 2 * NS) f[n + AHEAD] = value_operand(n + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+        if (more) {
+          settle(next, buf ^ 1);
+          __syncthreads();  // the next tile is in LDS, and this one's readers are done
+        }
+        now = next;
+        next = after;
       }
     }
     r.finish();
-    if (!SPLIT || (j0 == 0 && j1 == nt))
+    if (!split || (j0 == 0 && j1 == nt))
       r.write(a, F8 ? a.v_scale[hk] : 1.0f);
     else
       r.write_part(a, g * 2 + (first < u0 ? 0 : 1), TR, wave * 32 + (lane & 31));
-    if (!SPLIT) return;
+    if (!split) return;
     __syncthreads();  // the next row tile fills the buffers anew
     u += j1 - j0;
   }
@@ -715,22 +913,22 @@ bool usable(const hma_attn_paged_t* p) {
   return p->scale > 0.f && p->scale < 3e38f;
 }
 // Rule: sequences with at most 32 rows (tokens x shared heads) on average take the kernel whose waves share the keys, others the one
-// whose waves share the rows; the latter is split along the keys only where its row tiles do not give every compute unit its two
-// workgroups twice over.
+// whose waves share the rows: four waves, or eight with heads of 128 from 512 rows a sequence on.  The latter is split along the keys only
+// where its row tiles do not give every compute unit its workgroups twice over.
 Plan plan_of(const hma_attn_paged_t* p) {
   Plan r;
   const int64_t group = p->hq / p->hk, rows = p->tokens * group;
   r.few = rows <= 32LL * p->seqs;
   const int kb = p->d == 128 && !p->cache_e4m3 ? 1 : 2;
-  r.tr = r.few ? 32 : 128;
+  r.tr = r.few ? 32 : p->d == 128 && rows >= 512LL * p->seqs ? 256 : 128;
   r.tk = r.few ? WAVES * 32 * kb : 64;
   r.slots = rows / r.tr + p->seqs;
-  r.split = r.few || r.slots * p->hk < 4 * CUS;
-  // no more workgroups than units: row tiles x key tiles of the longest sequence that the table can hold
+  // as many workgroups as are resident together (their registers and LDS), each with one share, and no more than there are units: row
+  // tiles x key tiles of the longest sequence that the table can hold
+  const int64_t room = CUS * (r.few ? (p->d == 32 ? 3 : 2) : r.tr == 256 ? 1 : p->d == 128 ? 2 : p->d == 64 ? 3 : 4);
+  r.split = r.few || r.slots * p->hk < 2 * room;
   const int64_t most = ((int64_t)p->table_w * p->page + r.tk - 1) / r.tk;
   const int64_t units = r.slots * p->hk * (most > 0 ? most : 1);
-  // as many workgroups as are resident together (their registers and LDS), each with one share
-  const int64_t room = CUS * (r.few ? (p->d == 32 ? 3 : 2) : (p->d == 128 ? 2 : p->d == 64 ? 3 : 4));
   r.groups = (int)(units < room ? (units > 0 ? units : 1) : room);
   r.ws = r.split ? (int64_t)r.groups * 2 * r.tr * (p->d + 2) * 4 + (p->seqs + 2) * 8 : 0;
   return r;
@@ -744,7 +942,7 @@ int allow_lds() {
   if (hipGetDevice(&dev) != hipSuccess) return HMA_EINVAL;
   const uint64_t bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_relaxed) & bit) return 0;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 2 * 64 * (128 + PAD) * 2 + 4097 * 8);
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kern), hipFuncAttributeMaxDynamicSharedMemorySize, WAVES * 64 * (128 + PAD) * 2 + 4097 * 8);
   if (e != hipSuccess) return -(int)e;
   done.fetch_or(bit, std::memory_order_relaxed);
   return 0;
@@ -759,13 +957,15 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
     if (const int rc = allow_lds<attn_few_kernel<T, D, F8, KB, ALIGNED>>()) return rc;
     hipLaunchKernelGGL((attn_few_kernel<T, D, F8, KB, ALIGNED>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
   } else {
-    const size_t lds = (size_t)2 * 2 * 64 * LD * 2 + (r.split ? units : 0);
-    if (r.split) {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, true, ALIGNED>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, true, ALIGNED>), dim3((unsigned)r.groups), dim3(TPB), lds, st, a);
+    const size_t lds = (size_t)4 * Lay<D>::TILE + (r.split ? units : 0);
+    const dim3 grid((unsigned)(r.split ? r.groups : r.slots * a.hk));
+    constexpr int WIDE = D == 128 ? 8 : 4;
+    if (r.tr == 32 * WIDE) {
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, WIDE, ALIGNED>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, WIDE, ALIGNED>), grid, dim3(64 * WIDE), lds, st, a, (int)r.split);
     } else {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, false, ALIGNED>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, false, ALIGNED>), dim3((unsigned)(r.slots * a.hk)), dim3(TPB), lds, st, a);
+      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, 4, ALIGNED>>()) return rc;
+      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, 4, ALIGNED>), grid, dim3(TPB), lds, st, a, (int)r.split);
     }
   }
   HMA_CHECK_LAUNCH();
