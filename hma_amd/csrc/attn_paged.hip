@@ -94,7 +94,7 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
   const int64_t c0 = min(max((int64_t)a.cu[b], (int64_t)0), a.tokens), c1 = min(max((int64_t)a.cu[b + 1], c0), a.tokens);
   s.row0 = (int32_t)c0;
   s.n = (int32_t)(c1 - c0);
-  s.len = a.lens[b];
+  s.len = max(a.lens[b], -0x40000000);
   const int64_t room = min((int64_t)a.table_w * a.page, (int64_t)0x7fff0000);
   s.kv = a.pages > 0 ? (int32_t)min(max((int64_t)s.len, (int64_t)0), room) : 0;
   return s;

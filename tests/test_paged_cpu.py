@@ -1,0 +1,265 @@
+"""qk_rope, kv_append, attn_paged without a GPU: what the wrappers and the C entry points refuse, the shapes that tracing sees, the
+frequencies."""
+import contextlib
+import ctypes as C
+import math
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import hma_amd.torch_ops as T
+from hma_amd import _lib, ops
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+F8 = torch.float8_e4m3fn
+EINVAL = -10001
+
+
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The wrappers on host tensors, up to the launch."""
+    monkeypatch.setattr(ops, "_device", lambda *a: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "_stream", lambda t: 0)
+
+    def call(name, *a):
+        if name.endswith("_ws"):
+            return _lib.check(getattr(_lib.load(), name)(*a), name)
+        raise Launched(name)
+
+    monkeypatch.setattr(ops._lib, "call", call)
+
+
+def rope_args(**over):
+    a = dict(q=torch.zeros(5, 4, 32, dtype=BF), k=torch.zeros(5, 2, 32, dtype=BF), freqs=torch.ones(8, dtype=torch.float64), positions=torch.arange(5))
+    kw = dict(norm="rms", q_weight=torch.ones(32), k_weight=torch.ones(32))
+    for n, v in over.items():
+        (a if n in a else kw)[n] = v
+    return list(a.values()), kw
+
+
+ROPE_BAD = [dict(k=torch.zeros(6, 2, 32, dtype=BF)), dict(k=torch.zeros(5, 2, 16, dtype=BF)), dict(k=torch.zeros(5, 2, 32, dtype=HF)),
+            dict(q=torch.zeros(5, 4, 32, dtype=torch.float64), k=torch.zeros(5, 2, 32, dtype=torch.float64)), dict(q=torch.zeros(5, 128, dtype=BF)),
+            dict(freqs=torch.ones(8)), dict(freqs=torch.ones(17, dtype=torch.float64)), dict(freqs=torch.ones(4, 2, dtype=torch.float64)),
+            dict(positions=None), dict(positions=torch.arange(4)), dict(positions=torch.arange(5).float()),
+            dict(positions=torch.zeros(2, 5, dtype=torch.int64)), dict(positions=torch.arange(10)[::2]),
+            dict(axes=torch.zeros(8, dtype=torch.int64)), dict(axes=torch.zeros(7, dtype=torch.int32)),
+            dict(norm="batch"), dict(norm="none"), dict(q_weight=torch.ones(31)), dict(q_weight=torch.ones(32, dtype=HF), k_weight=None),
+            dict(q_weight=torch.ones(32, dtype=BF)), dict(q_bias=torch.zeros(32)), dict(q_weight=torch.ones(64)[::2])]
+
+
+@pytest.mark.parametrize("over", ROPE_BAD, ids=lambda o: "-".join(o))
+def test_qk_rope_refuses(host, over):
+    a, kw = rope_args(**over)
+    with pytest.raises(ValueError):
+        ops.qk_rope_fwd(*a, **kw)
+    a, kw = rope_args(**over)
+    with pytest.raises(ValueError):
+        ops.qk_rope_bwd(torch.zeros_like(a[0]), torch.zeros_like(a[1]), *a, **kw)
+
+
+def test_qk_rope_launches(host):
+    for over in (dict(), dict(norm="layer", q_bias=torch.zeros(32)), dict(norm="none", q_weight=None, k_weight=None, freqs=None, positions=None),
+                 dict(positions=torch.zeros(3, 5, dtype=torch.int32), axes=torch.zeros(8, dtype=torch.int32))):
+        a, kw = rope_args(**over)
+        with pytest.raises(Launched):
+            ops.qk_rope_fwd(*a, **kw)
+    a, kw = rope_args()
+    with pytest.raises(ValueError):
+        ops.qk_rope_bwd(torch.zeros(5, 4, 32), torch.zeros(5, 2, 32, dtype=BF), *a, **kw)
+
+
+def cache_args(**over):
+    a = dict(k=torch.zeros(3, 2, 32, dtype=BF), v=torch.zeros(3, 2, 32, dtype=BF), k_cache=torch.zeros(4, 2, 16, 32, dtype=BF),
+             v_cache=torch.zeros(4, 2, 16, 32, dtype=BF), page_table=torch.zeros(2, 3, dtype=torch.int32), cu_seqlens=torch.zeros(3, dtype=torch.int32),
+             kv_lens=torch.zeros(2, dtype=torch.int32))
+    kw = {}
+    for n, v in over.items():
+        (a if n in a else kw)[n] = v
+    return a, kw
+
+
+CACHE_BAD = [dict(k_cache=torch.zeros(4, 2, 16, 32, dtype=HF)), dict(v_cache=torch.zeros(4, 2, 8, 32, dtype=BF)),
+             dict(k_cache=torch.zeros(4, 2, 16, 32, dtype=F8), v_cache=torch.zeros(4, 2, 16, 32, dtype=F8)),  # no scales
+             dict(k_scale=torch.ones(2), v_scale=torch.ones(2)), dict(page_table=torch.zeros(2, 3, dtype=torch.int64)),
+             dict(page_table=torch.zeros(6, dtype=torch.int32)), dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t()),
+             dict(cu_seqlens=torch.zeros(2, dtype=torch.int32)), dict(kv_lens=torch.zeros(3, dtype=torch.int32)),
+             dict(cu_seqlens=torch.zeros(3, dtype=torch.int64)), dict(kv_lens=torch.zeros(4, dtype=torch.int32)[::2]),
+             dict(k_cache=torch.zeros(4, 2, 32, 16, dtype=BF).transpose(2, 3), v_cache=torch.zeros(4, 2, 32, 16, dtype=BF).transpose(2, 3))]
+E4M3 = dict(k_cache=torch.zeros(4, 2, 16, 32, dtype=F8), v_cache=torch.zeros(4, 2, 16, 32, dtype=F8))
+
+
+@pytest.mark.parametrize("over", CACHE_BAD + [dict(v=torch.zeros(3, 2, 16, dtype=BF)), dict(k=torch.zeros(3, 1, 32, dtype=BF), v=torch.zeros(3, 1, 32, dtype=BF)),
+                                              dict(k=torch.zeros(3, 2, 32), v=torch.zeros(3, 2, 32)), dict(q=torch.zeros(2, 4, 32, dtype=BF)),
+                                              dict(q=torch.zeros(3, 4, 32, dtype=HF)), dict(q_out=torch.zeros(3, 4, 32, dtype=BF)),
+                                              dict(q=torch.zeros(3, 4, 32, dtype=BF), q_out=torch.zeros(3, 4, 64, dtype=BF)[..., ::2]),
+                                              dict(norm="rms", q_weight=torch.ones(32)), dict(norm="rms", k_weight=torch.ones(16)),
+                                              E4M3 | dict(k_scale=torch.ones(2), v_scale=torch.ones(3)), E4M3 | dict(k_scale=torch.ones(2))],
+                         ids=lambda o: "-".join(o))
+def test_kv_append_refuses(host, over):
+    a, kw = cache_args(**over)
+    with pytest.raises(ValueError):
+        ops.kv_append(*a.values(), **kw)
+
+
+@pytest.mark.parametrize("over", CACHE_BAD + [dict(window=-1), dict(window=5, causal=False), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                                              dict(scale=math.inf), dict(q=torch.zeros(3, 3, 32, dtype=BF)), dict(q=torch.zeros(3, 4, 32)),
+                                              dict(q=torch.zeros(3, 4, 64, dtype=BF)), dict(out=torch.zeros(3, 4, 32, dtype=BF)),
+                                              dict(lse=torch.zeros(3, 4)), dict(out=torch.zeros(3, 4, 32, dtype=BF), lse=torch.zeros(3, 5)),
+                                              dict(out=torch.zeros(3, 4, 32, dtype=HF), lse=torch.zeros(3, 4))], ids=lambda o: "-".join(o))
+def test_attn_paged_refuses(host, over):
+    a, kw = cache_args(**over)
+    del a["k"], a["v"]
+    q, scale = kw.pop("q", torch.zeros(3, 4, 32, dtype=BF)), kw.pop("scale", 0.2)
+    with pytest.raises(ValueError):
+        ops.attn_paged_fwd(q, *a.values(), scale, **kw)
+
+
+def test_the_good_calls_launch(host):
+    a, kw = cache_args()
+    with pytest.raises(Launched):
+        ops.kv_append(*a.values())
+    a, kw = cache_args(**E4M3, k_scale=torch.ones(2), v_scale=torch.ones(2))
+    with pytest.raises(Launched):
+        ops.kv_append(*a.values(), **kw, q=torch.zeros(3, 4, 32, dtype=BF), norm="rms", q_weight=torch.ones(32))
+    del a["k"], a["v"]
+    with pytest.raises(Launched):
+        ops.attn_paged_fwd(torch.zeros(3, 4, 32, dtype=BF), *a.values(), 0.2, **kw)
+    with pytest.raises(NotImplementedError):
+        ops.attn_paged_fwd(torch.zeros(3, 4, 48, dtype=BF), *(torch.zeros(4, 2, 16, 48, dtype=BF),) * 2, *list(a.values())[2:], 0.2)
+
+
+def test_host_tensors_are_refused():
+    a, kw = rope_args()
+    with pytest.raises(RuntimeError):
+        ops.qk_rope_fwd(*a, **kw)
+    b, _ = cache_args()
+    with pytest.raises(RuntimeError):
+        ops.kv_append(*b.values())
+    with pytest.raises(RuntimeError):
+        ops.attn_paged_fwd(torch.zeros(3, 4, 32, dtype=BF), *list(b.values())[2:], 0.2)
+    with pytest.raises(NotImplementedError):
+        torch.ops.hma.qk_rope(a[0], a[1], a[2], a[3], None, False, 1.0, "none", None, None, None, None, 1e-5)
+
+
+# ------------------------------------------------------------------------------------------------ the C entry points
+def attn_struct(**over):
+    p = _lib.AttnPaged()
+    v = dict(q=16, o=16, lse=16, kc=16, vc=16, table=16, cu=16, lens=16, ws=16, ws_bytes=1 << 40, tokens=4, q_tok=128, q_head=32, kc_page=1024, kc_head=512,
+             kc_tok=32, vc_page=1024, vc_head=512, vc_tok=32, table_stride=4, hq=4, hk=2, d=32, dtype=0, seqs=2, table_w=4, pages=8, page=16, causal=1,
+             scale=0.2)
+    v.update(over)
+    for n, x in v.items():
+        setattr(p, n, x)
+    return p
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(q=18), dict(o=None), dict(o=8), dict(kc=None), dict(vc=8), dict(table=None), dict(cu=None), dict(lens=None),
+                                  dict(ws=None), dict(ws=8), dict(ws_bytes=64), dict(q_tok=4), dict(q_head=-32), dict(kc_page=1023), dict(vc_tok=4),
+                                  dict(kc_head=-512), dict(d=48), dict(d=256), dict(dtype=2), dict(hq=3), dict(hq=0), dict(hk=0), dict(seqs=-1),
+                                  dict(seqs=4097), dict(page=0), dict(pages=-1), dict(table_w=-1), dict(tokens=-1), dict(window=-1),
+                                  dict(window=4, causal=0), dict(scale=0.0), dict(scale=math.nan), dict(cache_e4m3=1),
+                                  dict(cache_e4m3=1, k_scale=16, v_scale=16, kc_tok=40)], ids=str)
+def test_attn_paged_entry_refuses(over):
+    assert _lib.load().hma_attn_paged_fwd(None, attn_struct(**over)) == EINVAL
+
+
+def test_attn_paged_workspace():
+    lib, n = _lib.load(), C.c_int64(-1)
+    assert lib.hma_attn_paged_ws(attn_struct(), None) == EINVAL and lib.hma_attn_paged_ws(None, C.byref(n)) == EINVAL
+    assert lib.hma_attn_paged_ws(attn_struct(), C.byref(n)) == 0 and n.value > 0
+    few = n.value
+    assert lib.hma_attn_paged_ws(attn_struct(table_w=4000), C.byref(n)) == 0 and n.value > few
+    assert lib.hma_attn_paged_ws(attn_struct(tokens=1 << 20), C.byref(n)) == 0 and n.value == 0  # nothing is split
+    assert lib.hma_attn_paged_fwd(None, attn_struct(tokens=0)) == 0  # nothing to do: no launch
+
+
+def rope_struct(cls, **over):
+    p = cls()
+    v = dict(tokens=4, hq=4, hk=2, q=16, k=16, q_tok=128, q_head=32, k_tok=64, k_head=32, q_out=16)
+    if cls is _lib.QkRope:
+        v |= dict(k_out=16, dy_q=16, dy_k=16, dyq_tok=128, dyq_head=32, dyk_tok=64, dyk_head=32, dq=16, dk=16)
+    else:
+        v |= dict(v=16, v_tok=64, v_head=32, kc=16, vc=16, kc_page=1024, kc_head=512, kc_tok=32, vc_page=1024, vc_head=512, vc_tok=32, table=16, cu=16,
+                  lens=16, table_stride=4, seqs=2, table_w=4, pages=8, page=16)
+    r = dict(freqs=16, positions=16, pos_stride=4, d=32, rot=16, norm=1, dtype=0, w_f32=1, pos_64=1, n_axes=1, eps=1e-5, amplitude=1.0)
+    for n, x in over.items():
+        (r if n in r or n in ("axes", "q_w", "q_b") else v)[n] = x
+    for n, x in v.items():
+        setattr(p, n, x)
+    for n, x in r.items():
+        setattr(p.r, n, x)
+    return p
+
+
+BAD_ROPE = [dict(d=12), dict(d=264), dict(d=0), dict(rot=15), dict(rot=34), dict(rot=-2), dict(freqs=None), dict(norm=3), dict(dtype=3), dict(hk=0), dict(tokens=-1),
+            dict(n_axes=0), dict(n_axes=2), dict(n_axes=2, axes=16, pos_stride=3), dict(norm=0, q_w=16), dict(k=None), dict(k=8), dict(k_tok=60), dict(k_head=-32),
+            dict(q=24), dict(q_tok=3), dict(q_out=None)]
+
+
+@pytest.mark.parametrize("over", BAD_ROPE, ids=str)
+def test_rope_entries_refuse(over):
+    lib = _lib.load()
+    assert lib.hma_qk_rope_fwd(None, rope_struct(_lib.QkRope, **over)) == EINVAL
+    if "q_out" not in over:
+        assert lib.hma_qk_rope_bwd(None, rope_struct(_lib.QkRope, **over)) == EINVAL
+    assert lib.hma_kv_append(None, rope_struct(_lib.KvAppend, **over)) == EINVAL
+
+
+def test_rope_entries_refuse_their_own():
+    lib = _lib.load()
+    assert lib.hma_qk_rope_fwd(None, rope_struct(_lib.QkRope, positions=None)) == EINVAL
+    assert lib.hma_qk_rope_fwd(None, rope_struct(_lib.QkRope, hq=0)) == EINVAL
+    assert lib.hma_qk_rope_fwd(None, None) == EINVAL and lib.hma_qk_rope_bwd(None, None) == EINVAL and lib.hma_kv_append(None, None) == EINVAL
+    for over in (dict(dq_w=16), dict(dq_w=16, ws=16, ws_floats=100), dict(dk=None), dict(dy_q=None), dict(dyk_tok=1), dict(norm=0, dq_b=16, ws=16, ws_floats=1 << 30)):
+        assert lib.hma_qk_rope_bwd(None, rope_struct(_lib.QkRope, **over)) == EINVAL
+    for over in (dict(dtype=2), dict(v=None), dict(v_tok=60), dict(page=0), dict(pages=-1), dict(seqs=-1), dict(table=None), dict(cu=None), dict(lens=None),
+                 dict(kc=None), dict(vc=8), dict(kc_tok=36), dict(vc_page=-8), dict(cache_e4m3=1), dict(cache_e4m3=1, k_scale=16, v_scale=16, kc=20)):
+        assert lib.hma_kv_append(None, rope_struct(_lib.KvAppend, **over)) == EINVAL, over
+    assert lib.hma_qk_rope_fwd(None, rope_struct(_lib.QkRope, tokens=0, positions=None)) == 0
+    assert lib.hma_kv_append(None, rope_struct(_lib.KvAppend, tokens=0)) == 0
+
+
+def test_struct_sizes_match_the_header():
+    assert C.sizeof(_lib.Rope) == 104 and C.sizeof(_lib.KvAppend) == 336 and C.sizeof(_lib.AttnPaged) == 232 and C.sizeof(_lib.QkRope) == 296
+
+
+# ------------------------------------------------------------------------------------------------ tracing, frequencies
+def test_fake_shapes():
+    assert {"qk_rope", "qk_rope_bwd", "kv_append", "attn_paged"} <= set(T.OPS)
+    with FakeTensorMode():
+        q, k = (torch.empty(5, h, 32, dtype=BF, device="cuda") for h in (4, 2))
+        f, w = torch.empty(8, dtype=torch.float64, device="cuda"), torch.empty(32, device="cuda")
+        pos = torch.empty(5, dtype=torch.int64, device="cuda")
+        y = torch.ops.hma.qk_rope(q, k, f, pos, None, False, 1.0, "rms", w, None, w, None, 1e-5)
+        assert [t.shape for t in y] == [q.shape, k.shape] and y[0].dtype == BF
+        y = torch.ops.hma.qk_rope(q.clone().requires_grad_(), k, f, pos, None, False, 1.0, "rms", w, None, w, None, 1e-5)
+        assert y[0].requires_grad
+        d = torch.ops.hma.qk_rope_bwd(q, k, q, k, f, pos, None, False, 1.0, "rms", w, None, w, None, 1e-5)
+        assert [t.shape for t in d] == [q.shape, k.shape, w.shape, w.shape]
+        kc = torch.empty(4, 2, 16, 32, dtype=BF, device="cuda")
+        tab, cu, lens = (torch.empty(s, dtype=torch.int32, device="cuda") for s in ((2, 3), (3,), (2,)))
+        out = torch.ops.hma.kv_append(k, k, kc, kc.clone(), tab, cu, lens, q, f, None, None, False, 1.0, "none", None, None, None, None, 1e-5, None, None)
+        assert out.shape == q.shape
+        o, lse = torch.ops.hma.attn_paged(q, kc, kc, tab, cu, lens, 0.2, True, 0, None, None)
+        assert o.shape == q.shape and lse.shape == (5, 4) and lse.dtype == F32
+
+
+def test_frequencies():
+    f, amp = ops.rope_freqs(64, 10000.0, device="cpu")
+    i = torch.arange(32, dtype=torch.float64)
+    assert torch.allclose(f, 10000.0 ** (-2 * i / 64), rtol=1e-14, atol=0) and amp == 1.0
+    assert torch.allclose(ops.rope_freqs(64, scaling="linear", factor=4.0, device="cpu")[0], f / 4, rtol=1e-14, atol=0)
+    base, _ = ops.rope_freqs(64, scaling="base", factor=4.0, device="cpu")
+    assert float(base[0]) == 1.0 and abs(float(base[-1] / f[-1]) - 0.25) < 1e-12
+    parts, amp = ops.rope_freqs(64, scaling="parts", factor=4.0, trained=4096, device="cpu")
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(parts[turns >= 32], f[turns >= 32]) and torch.allclose(parts[turns <= 1], f[turns <= 1] / 4, rtol=1e-14, atol=0)
+    assert bool((parts[1:] < parts[:-1]).all()) and abs(amp - (1 + 0.1 * math.log(4))) < 1e-12
+    for bad in (dict(rot=7), dict(rot=0), dict(rot=8, base=1.0), dict(rot=8, factor=0.0), dict(rot=8, scaling="other"), dict(rot=8, slow=4.0, fast=2.0)):
+        with pytest.raises(ValueError):
+            ops.rope_freqs(**bad, device="cpu")
