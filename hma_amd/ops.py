@@ -324,7 +324,7 @@ def attn_temporal_bwd(qkv, o, d_o, batch: int, T: int, n_s: int, scale: float):
 F8 = torch.float8_e4m3fn
 _DTYPE = {BF16: 0, torch.float16: 1, F32: 2}
 _NORM = {"none": 0, "rms": 1, "layer": 2}
-_QK_ROPE_WS_GROUPS = 1024
+_QK_ROPE_WS_GROUPS = 768
 
 
 _HERE = contextlib.nullcontext()

@@ -613,7 +613,7 @@ typedef struct {
 /* Forward: q [tokens][hq][d], k [tokens][hk][d] (strides in elements, the last one 1, rows 16-byte aligned) -> q_out, k_out
  * contiguous.  Backward: gradients dy_q, dy_k (strided alike) -> dq, dk contiguous; dq_w .. dk_b ([d] of the weights' type, NULL = not
  * wanted) are WRITTEN, summed in 32 bits in a fixed order through ws (HMA_QK_ROPE_WS_GROUPS * 4 * d floats, wanted only with them). */
-#define HMA_QK_ROPE_WS_GROUPS 1024
+#define HMA_QK_ROPE_WS_GROUPS 768
 typedef struct {
   hma_rope_t r;
   int64_t tokens; int32_t hq, hk;
