@@ -547,11 +547,11 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
   }
 }
 
-// ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 32 NW
-// The NW waves share tiles of 64 keys and values, two of each in LDS.  A wave has two companions at most on its SIMD and issues an
+// ------------------------------------------------------------------------------------- many rows: a wave takes 32 of the tile's 128
+// The waves share tiles of 64 keys and values, two of each in LDS.  A wave has two companions at most on its SIMD and issues an
 // instruction every five cycles or so, whatever its kind, so the instructions around the products and the exponentials are what there is
 // to save: 16-bit tiles come by LDS DMA in pieces of 1 KB, whose addresses are scalar (two lane reads and two additions a piece) plus one
-// register of lane offsets; a tile of keys is 16 such pieces at D = 128, two a wave.
+// register of lane offsets; a tile of keys is 16 such pieces at D = 128, four a wave.
 // Layout of a tile: piece = 64 / CPR rows (CPR = D / 8 chunks of 16 bytes each), pieces 16 bytes further apart than their size, chunk c of
 // row r at place c ^ turn(r) of its row.  A 16-byte read of 16 rows and a transposing read of 4 rows x 64 bytes then touch every bank once.
 template <int D>
@@ -560,12 +560,12 @@ struct Lay {
   static __device__ __forceinline__ int turn(int r) { return D == 128 ? 4 * (r & 3) : D == 64 ? 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1) : (r >> 2) & 3; }
   static __device__ __forceinline__ int at(int r, int c) { return r / RPP * PIECE + r % RPP * (2 * D) + (c ^ turn(r)) * 16; }
 };
-template <int D, int NW> struct ManyWaves { static constexpr int value = D == 128 ? 2 : D == 64 ? 3 : 4; };  // waves a SIMD
+template <int D> struct ManyWaves { static constexpr int value = D == 128 ? 2 : D == 64 ? 3 : 4; };  // waves a SIMD
 
-template <typename T, int D, bool F8, int NW, bool ALIGNED>
-__global__ __launch_bounds__(64 * NW, (ManyWaves<D, NW>::value)) void attn_many_kernel(const Args a, const int split) {
+template <typename T, int D, bool F8, bool ALIGNED>
+__global__ __launch_bounds__(TPB, ManyWaves<D>::value) void attn_many_kernel(const Args a, const int split) {
   typedef Lay<D> Y;
-  constexpr int TR = 32 * NW, TK = 64, BUF = 2 * Y::TILE, NO = D / 32;
+  constexpr int NW = WAVES, TR = 32 * NW, TK = 64, BUF = 2 * Y::TILE, NO = D / 32;
   constexpr bool DMA = !F8 && ALIGNED;
   constexpr int NP = Y::PIECES / NW;  // pieces of a tile per wave
   static_assert(Y::PIECES % NW == 0, "");
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(64 * NW, (ManyWaves<D, NW>::value)) void attn_many_
           // Two blocks of 32 keys.  The reads run AHEAD operands in front of the products that use them; the first block's exponentials stand
           // between the second's products, the second's between the first's values.  The barriers stop the compiler only: left alone it
           // puts each read right in front of its product and the exponentials behind the last, and the wave waits in both places.
-          constexpr int NS = D / 16, AHEAD = 4;  // operands of a block of 32 keys, of a block of 32 values
+          constexpr int NS = D / 16, AHEAD = 2;  // operands of a block of 32 keys, of a block of 32 values
           const auto key_operand = [&](int n) {
             const int at = D == 128 ? ka[(n % NS) >> 1] + (n & 1) * 32 : ka[n % NS % NKA];
             return *reinterpret_cast<const uint4*>(kt + at + n / NS * (32 / Y::RPP) * Y::PIECE);
@@ -745,6 +745,7 @@ __global__ __launch_bounds__(64 * NW, (ManyWaves<D, NW>::value)) void attn_many_
             const v4s16_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((HMA_LDS(v4s16_t)*)v8);
             return __builtin_bit_cast(uint4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
           };
+          __builtin_amdgcn_s_setprio(1);  // ahead of the SIMD's waves that wait or fetch (a frame of 320 tokens over 20k: 63 -> 61 us)
           const bool edge = key0 < w.lo_max || key0 + TK > w.hi_min || bad != 0;
           f32x16_t sc[2];
           uint4 f[2 * NS], p[2];
@@ -827,6 +828,7 @@ __global__ __launch_bounds__(64 * NW, (ManyWaves<D, NW>::value)) void attn_many_
             __builtin_amdgcn_sched_barrier(0);
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (more) {
           settle(next, buf ^ 1);
           __syncthreads();  // the next tile is in LDS, and this one's readers are done
@@ -913,19 +915,19 @@ bool usable(const hma_attn_paged_t* p) {
   return p->scale > 0.f && p->scale < 3e38f;
 }
 // Rule: sequences with at most 32 rows (tokens x shared heads) on average take the kernel whose waves share the keys, others the one
-// whose waves share the rows: four waves, or eight with heads of 128 from 512 rows a sequence on.  The latter is split along the keys only
-// where its row tiles do not give every compute unit its workgroups twice over.
+// whose waves share the rows.  The latter is split along the keys only where its row tiles do not give every compute unit its workgroups
+// twice over.
 Plan plan_of(const hma_attn_paged_t* p) {
   Plan r;
   const int64_t group = p->hq / p->hk, rows = p->tokens * group;
   r.few = rows <= 32LL * p->seqs;
   const int kb = p->d == 128 && !p->cache_e4m3 ? 1 : 2;
-  r.tr = r.few ? 32 : p->d == 128 && rows >= 512LL * p->seqs ? 256 : 128;
+  r.tr = r.few ? 32 : 128;
   r.tk = r.few ? WAVES * 32 * kb : 64;
   r.slots = rows / r.tr + p->seqs;
   // as many workgroups as are resident together (their registers and LDS), each with one share, and no more than there are units: row
   // tiles x key tiles of the longest sequence that the table can hold
-  const int64_t room = CUS * (r.few ? (p->d == 32 ? 3 : 2) : r.tr == 256 ? 1 : p->d == 128 ? 2 : p->d == 64 ? 3 : 4);
+  const int64_t room = CUS * (r.few ? (p->d == 32 ? 3 : 2) : p->d == 128 ? 2 : p->d == 64 ? 3 : 4);
   r.split = r.few || r.slots * p->hk < 2 * room;
   const int64_t most = ((int64_t)p->table_w * p->page + r.tk - 1) / r.tk;
   const int64_t units = r.slots * p->hk * (most > 0 ? most : 1);
@@ -959,14 +961,8 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
   } else {
     const size_t lds = (size_t)4 * Lay<D>::TILE + (r.split ? units : 0);
     const dim3 grid((unsigned)(r.split ? r.groups : r.slots * a.hk));
-    constexpr int WIDE = D == 128 ? 8 : 4;
-    if (r.tr == 32 * WIDE) {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, WIDE, ALIGNED>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, WIDE, ALIGNED>), grid, dim3(64 * WIDE), lds, st, a, (int)r.split);
-    } else {
-      if (const int rc = allow_lds<attn_many_kernel<T, D, F8, 4, ALIGNED>>()) return rc;
-      hipLaunchKernelGGL((attn_many_kernel<T, D, F8, 4, ALIGNED>), grid, dim3(TPB), lds, st, a, (int)r.split);
-    }
+    if (const int rc = allow_lds<attn_many_kernel<T, D, F8, ALIGNED>>()) return rc;
+    hipLaunchKernelGGL((attn_many_kernel<T, D, F8, ALIGNED>), grid, dim3(TPB), lds, st, a, (int)r.split);
   }
   HMA_CHECK_LAUNCH();
   if (r.split) {
