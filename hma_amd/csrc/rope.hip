@@ -5,7 +5,7 @@
 //   u = x  |  x / sqrt(mean x^2 + eps)  |  (x - mean x) / sqrt(var x + eps),
 // R rotates the first `rot` values in pairs -- (2 i, 2 i + 1) or (i, i + rot / 2) -- by the angle pos f_i and multiplies them by an
 // amplitude.  Written per value e with its pair's other value p(e):  R x[e] = x[e] C[e] + x[p(e)] S[e], S carrying the sign; the values
-// behind `rot` have C = 1, S = 0, so no lane branches.  R^T is the same with -S.
+// behind `rot` have C = 1, S = 0 and a zero as partner (an infinity behind `rot` stays one), so no lane branches.  R^T is the same with -S.
 //
 // Bound by the HBM bytes of the rows.  A lane holds 8 consecutive values of a row (16-byte loads and stores of 16-bit types), D / 8
 // lanes (rounded up to a power of two) hold a row, 64 lanes several heads: a unit, one load a lane.  What would bound it instead is the
@@ -218,7 +218,7 @@ __device__ __forceinline__ void rotate(const Shape& a, float* xch, int lane, int
   float p[8];
   if (INTER) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = x[e ^ 1];
+    for (int e = 0; e < 8; ++e) p[e] = e0 + e < a.rot ? x[e ^ 1] : 0.f;
   } else {
     float* mine = xch + lane * 8;
     *reinterpret_cast<float4*>(mine) = make_float4(x[0], x[1], x[2], x[3]);
@@ -231,13 +231,14 @@ __device__ __forceinline__ void rotate(const Shape& a, float* xch, int lane, int
       for (int q = 0; q < 8; q += 4) {
         const int e = e0 + q, at = e < half ? e + half : e < a.rot ? e - half : e;
         const float4 v = *reinterpret_cast<const float4*>(row + at);
-        p[q] = v.x; p[q + 1] = v.y; p[q + 2] = v.z; p[q + 3] = v.w;
+        const bool in = e < a.rot;
+        p[q] = in ? v.x : 0.f; p[q + 1] = in ? v.y : 0.f; p[q + 2] = in ? v.z : 0.f; p[q + 3] = in ? v.w : 0.f;
       }
     } else {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const int e = e0 + q, at = e < half ? e + half : e < a.rot ? e - half : e;
-        p[q] = row[at];
+        p[q] = e < a.rot ? row[at] : 0.f;
       }
     }
     wave_lds_order();  // the next rows are written behind these reads

@@ -237,6 +237,39 @@ def test_extremes():
     assert torch.equal(z[3], clean[3])
 
 
+@pytest.mark.parametrize("rot,inter", [(0, False), (24, False), (20, False), (20, True), (24, True), (2, True)])
+def test_values_behind_the_rotation_pass(rot, inter):
+    """An infinity, a NaN and the largest value behind `rot` come out as they went in and reach no other value, forward and backward."""
+    s = make(9, 3, 2, 64, rot, "none", BF, seed=12)
+    kw = dict(interleaved=inter)
+    clean = ops.qk_rope_fwd(s["q"], s["k"], s["freqs"], s["positions"], **kw)
+    q, k = s["q"].clone(), s["k"].clone()
+    for x in (q, k):
+        x[0, 0, rot], x[1, 1, rot + 1], x[2, 0, 63], x[3, 1, 63] = float("inf"), -float("inf"), float("nan"), torch.finfo(BF).max
+    odd = [x.float() != y.float() for x, y in ((q, s["q"]), (k, s["k"]))]
+    assert [int(o.sum()) for o in odd] == [4, 4]
+    clean_b = ops.qk_rope_bwd(s["q"], s["k"], s["q"], s["k"], s["freqs"], s["positions"], **kw)
+    got = ops.qk_rope_fwd(q, k, s["freqs"], s["positions"], **kw), ops.qk_rope_bwd(q, k, s["q"], s["k"], s["freqs"], s["positions"], **kw)
+    for ys, zs in zip(got, (clean, clean_b)):
+        for y, z, x, o in zip(ys, zs, (q, k), odd):
+            torch.testing.assert_close(y[o], x[o], rtol=0, atol=0, equal_nan=True)
+            assert torch.equal(y[~o], z[~o])
+
+
+def test_gradients_of_gradients_are_refused_and_broadcast_gradients_taken():
+    s = make(5, 2, 1, 32, 32, "rms", F32, seed=13)
+    q, k = s["q"].clone().requires_grad_(), s["k"].clone().requires_grad_()
+    y = torch.ops.hma.qk_rope(q, k, s["freqs"], s["positions"], None, False, 1.0, "rms", s["q_weight"], None, s["k_weight"], None, 1e-5)
+    gq, gk = torch.autograd.grad(y[0].sum() + y[1].sum(), [q, k], create_graph=True)  # a gradient with strides of zero
+    ones = [torch.ones_like(t) for t in y]
+    want = ops.qk_rope_bwd(*ones, s["q"], s["k"], s["freqs"], s["positions"], **kwargs(s, "rms", False, 1.0))
+    assert torch.equal(gq, want[0]) and torch.equal(gk, want[1])
+    y = torch.ops.hma.qk_rope(q, k, s["freqs"], s["positions"], None, False, 1.0, "rms", s["q_weight"], None, s["k_weight"], None, 1e-5)
+    gq, = torch.autograd.grad(y[0].square().sum() + y[1].sum(), [q], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        gq.square().sum().backward()
+
+
 # ------------------------------------------------------------------------------------------------ kv_append
 def paged(new, lens, page, hk, d, dtype, g, extra=2, tail=0):
     need = [-(-max(n, 0) // page) for n in lens]
