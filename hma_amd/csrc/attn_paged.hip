@@ -965,7 +965,7 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
     hipLaunchKernelGGL((attn_many_kernel<T, D, F8, ALIGNED>), grid, dim3(TPB), lds, st, a, (int)r.split);
   }
   HMA_CHECK_LAUNCH();
-  if (r.split) {
+  if (r.split && r.slots > 0) {  // (no sequences: none)
     const int most = (int)std::min<int64_t>(r.tr, a.tokens * a.group), per = TPB / (D / 4);
     hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(r.slots * a.hk), (unsigned)((most + per - 1) / per)), dim3(TPB), 0, st, a, r.tr, r.tk);
     HMA_CHECK_LAUNCH();

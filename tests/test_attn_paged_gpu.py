@@ -182,6 +182,46 @@ def test_what_no_row_of_a_tile_sees_is_not_read():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 300])
+def test_no_sequences(tokens):
+    s = batch([], [], 16, 4, 2, 32, BF, tail=tokens)
+    o, lse = call(s, 0.2)
+    assert o.shape == (tokens, 4, 32) and not o.any() and bool((lse == -math.inf).all())
+    mine = torch.full_like(o, 3.0), torch.full_like(lse, 3.0)
+    call(s, 0.2, out=mine[0], lse=mine[1])
+    assert bool((mine[0] == 3).all() and (mine[1] == 3).all())
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("new,lens", [([1, 1], [300, 77]), ([200, 70], [500, 70]), ([3000], [3000])])
+def test_rows_that_are_no_numbers_stay_their_own(new, lens, d):
+    """A query row with a NaN or an infinity: NaN there (one key's score is a NaN or both signs are infinite), every other row as without."""
+    s = batch(new, lens, 16, 4, 2, d, BF, seed=13)
+    want = call(s, 0.125)
+    q = s["q"].clone()
+    q[0, 0], q[-1, 3], q[-1, 1, 5] = float("nan"), float("inf"), float("nan")
+    o, lse = call(dict(s, q=q), 0.125)
+    odd = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    odd[0, 0] = odd[-1, 3] = odd[-1, 1] = True
+    assert bool(o[odd].isnan().all()) and bool(lse[odd].isnan().all())
+    assert torch.equal(o[~odd], want[0][~odd]) and torch.equal(lse[~odd], want[1][~odd])
+
+
+def test_two_calls_at_once():
+    a, b = batch([1, 1, 1], [700, 900, 333], 16, 8, 2, 128, BF, seed=14), batch([140, 2], [700, 500], 16, 8, 2, 128, BF, seed=15)
+    want = [call(x, 0.09) for x in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(x, 0.09))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g[0], want[i][0]) and torch.equal(g[1], want[i][1]) for g in got[i])
+
+
 def test_strides_and_streams():
     s = batch([3, 1, 200], [70, 300, 333], 16, 8, 4, 64, BF, seed=8)
     want = call(s, 0.125)
