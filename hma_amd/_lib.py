@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhma_hip.so")
@@ -217,6 +218,19 @@ class AttnPaged(C.Structure):
         ("cache_e4m3", c_i32), ("causal", c_i32), ("window", c_i32), ("zero_tail", c_i32),
         ("scale", c_f32), ("_pad", c_i32),
     ]
+
+
+def packer(cls) -> struct.Struct:
+    """The fields of `cls`, nested ones in their place, as one struct format: pack_into(instance, 0, *values) fills all of them in one call
+    (None is no pointer: pass 0)."""
+    code = {c_vp: "P", c_i64: "q", c_i32: "i", c_f32: "f"}
+
+    def fields(c):
+        return "".join(code[t] if t in code else fields(t) for _, t in c._fields_)
+
+    s = struct.Struct("@" + fields(cls))
+    assert s.size == C.sizeof(cls)
+    return s
 
 
 _PROTOS = {

@@ -327,6 +327,10 @@ _NORM = {"none": 0, "rms": 1, "layer": 2}
 _QK_ROPE_WS_GROUPS = 768
 
 
+# These wrappers stand in front of launches of a few microseconds: an argument structure is filled in one call (setting its 50 fields one by
+# one took longer than the launch)
+_QK_ROPE, _KV_APPEND, _ATTN_PAGED = (_lib.packer(c) for c in (QkRope, KvAppend, AttnPaged))
+_NO_GRADIENTS = (0,) * 14  # the fields of QkRope behind k_out
 _HERE = contextlib.nullcontext()
 
 
@@ -350,6 +354,10 @@ def _stream(t: torch.Tensor) -> int:
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -387,51 +395,49 @@ def rope_freqs(rot: int, base: float = 10000.0, *, scaling: str = "none", factor
     return f.to(device), amplitude
 
 
-def _fill_rope(r, dtype, d: int, tokens: int, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps) -> None:
-    rot = 0
+# hma_rope_t in the order of its fields
+def _rope_values(dtype, d: int, tokens: int, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps) -> tuple:
+    rot, f, a, at, pos64, n_axes, pos_stride = 0, 0, 0, 0, 0, 1, 0
     if freqs is not None:
-        _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and 2 * freqs.numel() <= d,
-              "freqs: float64 (rot / 2,) contiguous, rot <= head size")
         rot = 2 * freqs.numel()
-        r.freqs = freqs.data_ptr()
-    r.n_axes = 1
+        _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and rot <= d, "freqs: float64 (rot / 2,) contiguous, rot <= head size")
+        f = freqs.data_ptr()
     if positions is not None and rot:
-        _need(positions.dtype in (torch.int64, torch.int32) and positions.dim() in (1, 2) and positions.shape[-1] == tokens and
-              (tokens <= 1 or positions.stride(-1) == 1), "positions: int64 or int32, (tokens,) or (axes, tokens), contiguous over the tokens")
-        r.positions, r.pos_64 = positions.data_ptr(), positions.dtype == torch.int64
-        if positions.dim() == 2:
-            _need(positions.shape[0] >= 1 and (axes is not None or positions.shape[0] == 1) and (positions.shape[0] == 1 or positions.stride(0) >= tokens),
+        shape, stride, kind = positions.shape, positions.stride(), positions.dtype
+        pos64 = kind == torch.int64
+        _need((pos64 or kind == torch.int32) and len(shape) in (1, 2) and shape[-1] == tokens and (tokens <= 1 or stride[-1] == 1),
+              "positions: int64 or int32, (tokens,) or (axes, tokens), contiguous over the tokens")
+        at = positions.data_ptr()
+        if len(shape) == 2:
+            n_axes, pos_stride = shape[0], stride[0]
+            _need(n_axes >= 1 and (axes is not None or n_axes == 1) and (n_axes == 1 or pos_stride >= tokens),
                   "positions of several axes need `axes` and rows that do not overlap")
-            r.n_axes, r.pos_stride = positions.shape[0], positions.stride(0)
     if axes is not None and rot:
         _need(axes.dtype == torch.int32 and axes.shape == freqs.shape and axes.is_contiguous(), "axes: int32 (rot / 2,) contiguous")
-        r.axes = axes.data_ptr()
-    if norm not in _NORM:
+        a = axes.data_ptr()
+    kind = _NORM.get(norm)
+    if kind is None:
         raise ValueError(f"norm {norm!r}: none, rms or layer")
-    wt = None
-    for w in (q_weight, q_bias, k_weight, k_bias):
-        if w is not None:
-            _need(norm != "none" and w.shape == (d,) and w.is_contiguous() and w.dtype in (F32, dtype) and wt in (None, w.dtype),
+    w, wt = [0, 0, 0, 0], None
+    for i, t in enumerate((q_weight, q_bias, k_weight, k_bias)):
+        if t is not None:
+            _need(kind and t.shape == (d,) and t.is_contiguous() and t.dtype in (F32, dtype) and wt in (None, t.dtype),
                   "norm weights: (head size,) contiguous, all fp32 or all of the rows' type, with a norm")
-            wt = w.dtype
-    _need(norm == "layer" or (q_bias is None and k_bias is None), "a bias goes with norm 'layer'")
-    r.q_w, r.q_b, r.k_w, r.k_b = ptr(q_weight), ptr(q_bias), ptr(k_weight), ptr(k_bias)
-    r.w_f32 = wt in (None, F32)
-    r.d, r.rot, r.interleaved, r.norm, r.dtype, r.eps, r.amplitude = d, rot, bool(interleaved), _NORM[norm], _DTYPE[dtype], eps, amplitude
+            wt = t.dtype
+            w[i] = t.data_ptr()
+    _need(kind == 2 or (q_bias is None and k_bias is None), "a bias goes with norm 'layer'")
+    return f, a, at, pos_stride, *w, d, rot, bool(interleaved), kind, _DTYPE[dtype], wt in (None, F32), pos64, n_axes, eps, amplitude
 
 
-def _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps):
-    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and q.dtype == k.dtype and q.dtype in _DTYPE,
+def _qk_values(q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps):
+    """q, k as the kernels read them, and the first fields of hma_qk_rope_t"""
+    kind, qs, ks = q.dtype, q.shape, k.shape
+    _need(len(qs) == 3 and len(ks) == 3 and qs[0] == ks[0] and qs[2] == ks[2] and kind == k.dtype and kind in _DTYPE,
           "q (tokens, heads, d) and k (tokens, kv heads, d) of one type: bf16, fp16 or fp32")
     _need(freqs is None or positions is not None, "a rotation needs positions")
     q, k = _rows16(q), _rows16(k)
-    tokens, p.hq, d = q.shape
-    p.tokens, p.hk = tokens, k.shape[1]
-    _fill_rope(p.r, q.dtype, d, tokens, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
-    p.q, p.k = q.data_ptr(), k.data_ptr()
-    p.q_tok, p.q_head, _ = q.stride()
-    p.k_tok, p.k_head, _ = k.stride()
-    return q, k
+    rope = _rope_values(kind, qs[2], qs[0], freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+    return q, k, (*rope, qs[0], qs[1], ks[1], q.data_ptr(), k.data_ptr(), *q.stride()[:2], *k.stride()[:2])
 
 
 def qk_rope_fwd(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor], positions: Optional[torch.Tensor], *, axes: Optional[torch.Tensor] = None,
@@ -441,11 +447,11 @@ def qk_rope_fwd(q: torch.Tensor, k: torch.Tensor, freqs: Optional[torch.Tensor],
     its first 2 * len(freqs) values by positions * freqs, in one pass (hma_qk_rope_fwd).  bf16, fp16 or fp32; d a multiple of 8 up to 256;
     views of a packed projection need no copy.  positions (tokens,) or (axes, tokens) with `axes` int32 naming each pair's axis.  Returns
     contiguous (q, k)."""
-    p = QkRope()
     with _device(q, k, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias):
-        qr, kr = _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        qr, kr, values = _qk_values(q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
         qo, ko = _like(q), _like(k)
-        p.q_out, p.k_out = qo.data_ptr(), ko.data_ptr()
+        p = QkRope()
+        _QK_ROPE.pack_into(p, 0, *values, qo.data_ptr(), ko.data_ptr(), *_NO_GRADIENTS)
         _lib.call("hma_qk_rope_fwd", _stream(q), C.byref(p))
     return qo, ko
 
@@ -454,46 +460,41 @@ def qk_rope_bwd(dy_q: torch.Tensor, dy_k: torch.Tensor, q: torch.Tensor, k: torc
                 amplitude: float = 1.0, norm: str = "none", q_weight=None, q_bias=None, k_weight=None, k_bias=None, eps: float = 1e-5):
     """(dq, dk, d q_weight, d q_bias, d k_weight, d k_bias) of qk_rope_fwd from its inputs and the gradients of its outputs; the weights'
     gradients (None where there is no weight) are summed in 32 bits in a fixed order (hma_qk_rope_bwd)."""
-    p = QkRope()
     with _device(q, k, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias, dy_q, dy_k):
         _need(dy_q.shape == q.shape and dy_k.shape == k.shape and dy_q.dtype == q.dtype and dy_k.dtype == k.dtype, "gradients of the shapes and type of q and k")
-        qr, kr = _fill_qk(p, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        qr, kr, values = _qk_values(q, k, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
         gq, gk = _rows16(dy_q), _rows16(dy_k)
-        p.dy_q, p.dy_k = gq.data_ptr(), gk.data_ptr()
-        p.dyq_tok, p.dyq_head, _ = gq.stride()
-        p.dyk_tok, p.dyk_head, _ = gk.stride()
         dq, dk = _like(q), _like(k)
         dw = [None if w is None else torch.empty_like(w) for w in (q_weight, q_bias, k_weight, k_bias)]
-        p.dq, p.dk = dq.data_ptr(), dk.data_ptr()
-        p.dq_w, p.dq_b, p.dk_w, p.dk_b = (ptr(w) for w in dw)
-        ws = None
-        if any(w is not None for w in dw):
-            ws = torch.empty(_QK_ROPE_WS_GROUPS * 4 * q.shape[2], dtype=F32, device=q.device)
-            p.ws, p.ws_floats = ws.data_ptr(), ws.numel()
+        ws = torch.empty(_QK_ROPE_WS_GROUPS * 4 * q.shape[2], dtype=F32, device=q.device) if any(w is not None for w in dw) else None
+        p = QkRope()
+        _QK_ROPE.pack_into(p, 0, *values, 0, 0, gq.data_ptr(), gk.data_ptr(), *gq.stride()[:2], *gk.stride()[:2], dq.data_ptr(), dk.data_ptr(),
+                           *(_at(w) for w in dw), _at(ws), 0 if ws is None else ws.numel())
         _lib.call("hma_qk_rope_bwd", _stream(q), C.byref(p))
     return (dq, dk, *dw)
 
 
-def _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, dtype) -> None:
-    """The paged cache of hma_kv_append / hma_attn_paged_fwd: caches (pages, kv heads, page size, d), table int32 (sequences, pages of one)."""
-    pages, hk, page, d = k_cache.shape
-    _need(v_cache.shape == k_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.dtype in (dtype, F8) and page > 0,
+def _cache_values(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, dtype) -> tuple:
+    """The paged cache of hma_kv_append / hma_attn_paged_fwd: caches (pages, kv heads, page size, d), table int32 (sequences, pages of one).
+    ((both caches, table, cu, lens, scales), (strides of both caches), stride of the table, (sequences, table's width, pages, page size, e4m3))"""
+    shape, kind, table = k_cache.shape, k_cache.dtype, page_table.shape
+    f8 = kind == F8
+    _need(len(shape) == 4 and v_cache.shape == shape and v_cache.dtype == kind and (f8 or kind == dtype) and shape[2] > 0,
           "caches: (pages, kv heads, page size, d), both of the rows' type or both float8_e4m3fn")
-    _need(page_table.dim() == 2 and cu_seqlens.shape == (page_table.shape[0] + 1,) and kv_lens.shape == (page_table.shape[0],) and
-          page_table.dtype == cu_seqlens.dtype == kv_lens.dtype == torch.int32 and cu_seqlens.is_contiguous() and kv_lens.is_contiguous() and
-          (page_table.shape[1] <= 1 or page_table.stride(1) == 1), "page_table (sequences, n), cu_seqlens (sequences + 1,), kv_lens (sequences,): int32")
-    f8 = k_cache.dtype == F8
-    _need((k_scale is not None and v_scale is not None) if f8 else (k_scale is None and v_scale is None), "scales go with a float8_e4m3fn cache, and only with it")
+    _need(len(table) == 2 and cu_seqlens.shape == (table[0] + 1,) and kv_lens.shape == (table[0],) and
+          page_table.dtype == cu_seqlens.dtype == kv_lens.dtype == torch.int32 and cu_seqlens.is_contiguous() and kv_lens.is_contiguous(),
+          "page_table (sequences, n), cu_seqlens (sequences + 1,), kv_lens (sequences,): int32")
+    t0, t1 = page_table.stride()
+    _need(table[1] <= 1 or t1 == 1, "page_table: a sequence's pages one behind the other")
+    _need((k_scale is None) == (v_scale is None) == (not f8), "scales go with a float8_e4m3fn cache, and only with it")
     if f8:
         for s in (k_scale, v_scale):
-            _need(s.dtype == F32 and s.shape == (hk,) and s.is_contiguous(), "k_scale, v_scale: fp32 (kv heads,) contiguous")
-        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-    p.kc, p.vc, p.cache_e4m3 = k_cache.data_ptr(), v_cache.data_ptr(), f8
-    p.kc_page, p.kc_head, p.kc_tok, one = k_cache.stride()
-    p.vc_page, p.vc_head, p.vc_tok, two = v_cache.stride()
-    _need(one == 1 and two == 1, "the caches' last dimension is contiguous")
-    p.table, p.cu, p.lens, p.table_stride = page_table.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), page_table.stride(0)
-    p.seqs, p.table_w, p.pages, p.page = page_table.shape[0], page_table.shape[1], pages, page
+            _need(s.dtype == F32 and s.shape == shape[1:2] and s.is_contiguous(), "k_scale, v_scale: fp32 (kv heads,) contiguous")
+    k0, k1, k2, k3 = k_cache.stride()
+    v0, v1, v2, v3 = v_cache.stride()
+    _need(k3 == 1 and v3 == 1, "the caches' last dimension is contiguous")
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), cu_seqlens.data_ptr(), kv_lens.data_ptr(), _at(k_scale), _at(v_scale)),
+            (k0, k1, k2, v0, v1, v2), t0, (table[0], table[1], shape[0], shape[2], f8))
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -506,28 +507,30 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     page_table[b, p // page size].  positions None: a token's place.  float8_e4m3fn caches store x / scale[head].  With q (tokens, heads,
     d): returns q normed and rotated (rows behind the last sequence zero; with q_out given they are left as they were).  A token without a
     place (kv_lens too small, a page number outside the cache) is not stored.  Pages written by one call belong to one sequence each."""
-    p = KvAppend()
     with _device(k, v, k_cache, v_cache, page_table, cu_seqlens, kv_lens, q, freqs, positions, axes, q_weight, q_bias, k_weight, k_bias, k_scale,
                  v_scale, q_out):
-        _need(k.dim() == 3 and v.shape == k.shape and k.dtype == v.dtype and k.dtype in (BF16, torch.float16), "k, v: (tokens, kv heads, d) of one type, bf16 or fp16")
-        tokens, p.hk, d = k.shape
-        p.tokens = tokens
-        _need(k_cache.dim() == 4 and k_cache.shape[1] == p.hk and k_cache.shape[3] == d, "caches of k's heads and head size")
-        _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, k.dtype)
-        _fill_rope(p.r, k.dtype, d, tokens, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
+        kind, shape = k.dtype, k.shape
+        _need(len(shape) == 3 and v.shape == shape and v.dtype == kind and (kind == BF16 or kind == torch.float16), "k, v: (tokens, kv heads, d) of one type, bf16 or fp16")
+        tokens, hk, d = shape
+        (kc, vc, *lists), strides, table_stride, sizes = _cache_values(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, kind)
+        _need(k_cache.shape[1] == hk and k_cache.shape[3] == d, "caches of k's heads and head size")
+        rope = _rope_values(kind, d, tokens, freqs, positions, axes, interleaved, amplitude, norm, q_weight, q_bias, k_weight, k_bias, eps)
         _need(q is not None or (q_weight is None and q_bias is None and q_out is None), "q's weights and output without q")
         k, v = _rows16(k), _rows16(v)
-        p.k, p.v = k.data_ptr(), v.data_ptr()
-        p.k_tok, p.k_head, _ = k.stride()
-        p.v_tok, p.v_head, _ = v.stride()
+        hq, q_at, q_to, q_tok, q_head, zero_tail = 0, 0, 0, 0, 0, 0
         if q is not None:
-            _need(q.dim() == 3 and q.shape[0] == tokens and q.shape[2] == d and q.dtype == k.dtype, "q: (tokens, heads, d) of k's type")
+            qs = q.shape
+            _need(len(qs) == 3 and qs[0] == tokens and qs[2] == d and q.dtype == kind, "q: (tokens, heads, d) of k's type")
             if q_out is None:
-                q_out, p.zero_tail = _like(q), 1
-            _need(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.is_contiguous(), "q_out: q's shape and type, contiguous")
+                q_out, zero_tail = _like(q), 1
+            else:
+                _need(q_out.shape == qs and q_out.dtype == kind and q_out.is_contiguous(), "q_out: q's shape and type, contiguous")
             q = _rows16(q)
-            p.q, p.q_out, p.hq = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-            p.q_tok, p.q_head, _ = q.stride()
+            hq, q_at, q_to = qs[1], q.data_ptr(), q_out.data_ptr()
+            q_tok, q_head, _ = q.stride()
+        p = KvAppend()
+        _KV_APPEND.pack_into(p, 0, *rope, tokens, hq, hk, q_at, k.data_ptr(), v.data_ptr(), q_tok, q_head, *k.stride()[:2], *v.stride()[:2], q_to,
+                             kc, vc, *strides, *lists[:3], table_stride, *lists[3:], *sizes, zero_tail)
         _lib.call("hma_kv_append", _stream(k), C.byref(p))
     return q_out
 
@@ -540,28 +543,31 @@ def attn_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     sequence (causal=False: a chunk whose tokens see each other, such as a frame).  bf16 or fp16, d 32, 64 or 128, heads a multiple of
     the cache's; a cache of q's type or float8_e4m3fn with scales (hma_attn_paged_fwd).  lse fp32 (tokens, heads); a row that sees no key has o = 0,
     lse = -inf, and so have rows behind the last sequence (with out / lse given those are left as they were)."""
-    p = AttnPaged()
     with _device(q, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, out, lse):
-        _need(q.dim() == 3 and q.dtype in (BF16, torch.float16) and k_cache.dim() == 4 and k_cache.shape[3] == q.shape[2] and k_cache.shape[1] > 0 and
-              q.shape[1] % k_cache.shape[1] == 0, "q: (tokens, heads, d) bf16 or fp16, heads a multiple of the cache's, d the cache's")
-        if q.shape[2] not in (32, 64, 128):
+        kind, shape, cache = q.dtype, q.shape, k_cache.shape
+        _need(len(shape) == 3 and (kind == BF16 or kind == torch.float16) and len(cache) == 4 and cache[3] == shape[2] and cache[1] > 0 and
+              shape[1] % cache[1] == 0, "q: (tokens, heads, d) bf16 or fp16, heads a multiple of the cache's, d the cache's")
+        tokens, hq, d = shape
+        if d not in (32, 64, 128):
             raise NotImplementedError("attn_paged is built for heads of 32, 64 and 128")
         _need(window >= 0 and (causal or window == 0), "a window goes with causal")
         _need(0 < scale < 3e38, "scale > 0")
-        _fill_cache(p, k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, q.dtype)
+        lists, strides, table_stride, sizes = _cache_values(k_cache, v_cache, page_table, cu_seqlens, kv_lens, k_scale, v_scale, kind)
         q = _rows16(q)
-        p.tokens, p.hq, p.d = q.shape
-        p.hk, p.dtype, p.causal, p.window, p.scale = k_cache.shape[1], _DTYPE[q.dtype], causal, window, scale
-        p.q_tok, p.q_head, _ = q.stride()
         _need((out is None) == (lse is None), "out and lse together")
-        if out is None:
-            out, lse, p.zero_tail = _like(q), q.new_empty(q.shape[:2], dtype=F32), 1
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and lse.shape == q.shape[:2] and lse.dtype == F32 and
-              lse.is_contiguous(), "out: q's shape and type, lse: fp32 (tokens, heads), contiguous")
-        p.q, p.o, p.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
-        n = C.c_int64()
+        zero_tail = out is None
+        if zero_tail:
+            out, lse = _like(q), torch.empty(shape[:2], dtype=F32, device=q.device)
+        else:
+            _need(out.shape == shape and out.dtype == kind and out.is_contiguous() and lse.shape == shape[:2] and lse.dtype == F32 and
+                  lse.is_contiguous(), "out: q's shape and type, lse: fp32 (tokens, heads), contiguous")
+        q_tok, q_head, _ = q.stride()
+        p, n = AttnPaged(), C.c_int64()
+        _ATTN_PAGED.pack_into(p, 0, q.data_ptr(), out.data_ptr(), lse.data_ptr(), *lists, 0, 0, tokens, q_tok, q_head, *strides, table_stride, hq, cache[1], d,
+                              _DTYPE[kind], *sizes, causal, window, zero_tail, scale, 0)
         _lib.call("hma_attn_paged_ws", C.byref(p), C.byref(n))
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device) if n.value else None
-        p.ws, p.ws_bytes = ptr(ws), n.value
+        if n.value:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+            p.ws, p.ws_bytes = ws.data_ptr(), n.value
         _lib.call("hma_attn_paged_fwd", _stream(q), C.byref(p))
     return out, lse
