@@ -89,16 +89,17 @@ __device__ __forceinline__ void wave_lds_order() {
 struct Seq {
   int32_t row0, n, kv, len;  // first row of the batch, new tokens, keys that the table can hold, length
 };
-__device__ __forceinline__ Seq seq_of(const Args& a, int b) {
+__device__ __forceinline__ Seq seq_from(const Args& a, int cu0, int cu1, int len) {
   Seq s;
-  const int64_t c0 = min(max((int64_t)a.cu[b], (int64_t)0), a.tokens), c1 = min(max((int64_t)a.cu[b + 1], c0), a.tokens);
+  const int64_t c0 = min(max((int64_t)cu0, (int64_t)0), a.tokens), c1 = min(max((int64_t)cu1, c0), a.tokens);
   s.row0 = (int32_t)c0;
   s.n = (int32_t)(c1 - c0);
-  s.len = max(a.lens[b], -0x40000000);
+  s.len = max(len, -0x40000000);
   const int64_t room = min((int64_t)a.table_w * a.page, (int64_t)0x7fff0000);
   s.kv = a.pages > 0 ? (int32_t)min(max((int64_t)s.len, (int64_t)0), room) : 0;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const Args& a, int b) { return seq_from(a, a.cu[b], a.cu[b + 1], a.lens[b]); }
 __device__ __forceinline__ int row_tiles(const Args& a, const Seq& s, int tr) { return (int)(((int64_t)s.n * a.group + tr - 1) / tr); }
 // key tiles of a row tile: the most that any of the sequence's row tiles needs, one at least (a row that sees nothing is written too)
 __device__ __forceinline__ int key_tiles(const Args& a, const Seq& s, int tr, int tk) {
@@ -139,7 +140,8 @@ __device__ __forceinline__ void unit_table(const Args& a, int64_t* base, int64_t
 
 // Row tile numbers: sequence b owns first_slot(b) .. first_slot(b + 1) - 1, at least as many as it needs, known without a sum over the
 // sequences.  The sequence of a number by the whole wave, 64 candidates a step.
-__device__ __forceinline__ int64_t first_slot(const Args& a, int b, int tr) { return (int64_t)a.cu[b] * a.group / tr + b; }
+__device__ __forceinline__ int64_t slot_from(const Args& a, int cu, int b, int tr) { return (int64_t)cu * a.group / tr + b; }
+__device__ __forceinline__ int64_t first_slot(const Args& a, int b, int tr) { return slot_from(a, a.cu[b], b, tr); }
 __device__ __forceinline__ int seq_of_slot(const Args& a, int64_t slot, int tr) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = a.seqs;
@@ -653,7 +655,18 @@ __global__ __launch_bounds__(TPB, ManyWaves<D>::value) void attn_many_kernel(con
     uint4 kr[DMA ? 1 : NI], vr[DMA ? 1 : NI];
     // tile of `p` on its way: into LDS buffer `buf`, or into registers
     const auto fetch = [&](const Place& p, int buf) {
-      if (DMA) {
+      if (DMA && NP <= 2) {  // few pieces a wave: their addresses by scalar products (D = 32, a frame: 52.7 -> 51.2 us)
+        const int raw = p.good(a) ? p.raw : 0, off = p.good(a) ? p.off : 0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int piece = i * NW + wave, row = piece * Y::RPP;
+          const int64_t pg = __builtin_amdgcn_readlane(raw, row), of = __builtin_amdgcn_readlane(off, row);
+          const uint32_t to = lds0 + buf * BUF + piece * Y::PIECE;
+          const int64_t ko = pg * a.kc_page + of * a.kc_tok;
+          glds16s(kc + ko, k_off, to);
+          glds16s(vc + (alike ? ko : pg * a.vc_page + of * a.vc_tok), v_off, to + Y::TILE);
+        }
+      } else if (DMA) {
         const int64_t ko = p.at(a, a.kc_page, a.kc_tok);
         int64_t vo = ko;
         if (!alike) vo = p.at(a, a.vc_page, a.vc_tok);
@@ -850,15 +863,36 @@ __global__ __launch_bounds__(TPB, ManyWaves<D>::value) void attn_many_kernel(con
 
 // ------------------------------------------------------------------------------------- joining shared row tiles
 // A workgroup joins as many rows of a (row tile, key head) as its threads hold, D / 4 threads a row; blockIdx.y walks the tile's rows.  The
-// shares of a row are loaded eight at a time: the launch is short and all latency.
+// launch is short and all latency: where the row tile lies comes in one trip to memory, up to eight shares of a row are loaded together.
+// 10 shares of 96 tiles of 128 rows x 32 (17 MB): 6.7 us; 4 or 16 at a time 7.0 and 7.3, shares that are not there loaded all the same 8.4.
 template <typename T, int D>
 __global__ __launch_bounds__(TPB) void attn_join_kernel(const Args a, int tr, int tk) {
   constexpr int TPR = D / 4, RPB = TPB / TPR, AT = 8;
   const int64_t slot = blockIdx.x / a.hk;
-  const int hk = blockIdx.x % a.hk, b = seq_of_slot(a, slot, tr);
-  if (b >= a.seqs) return;
-  const Seq s = seq_of(a, b);
-  const int64_t qt = slot - first_slot(a, b, tr), each = a.units[a.seqs + 1], base = a.units[b];
+  const int hk = blockIdx.x % a.hk;
+  const int64_t each = a.units[a.seqs + 1];
+  int b, cu0, cu1, len;
+  int64_t base;
+  if (a.seqs <= 64) {  // every sequence in a lane: one trip to memory instead of three
+    const int lane = threadIdx.x & 63, at = min(lane, max(a.seqs - 1, 0));
+    const int c0 = a.cu[at], c1 = a.cu[min(at + 1, a.seqs)], l = a.lens[at];
+    const int64_t u = a.units[at];
+    b = __popcll(__ballot(lane < a.seqs && slot_from(a, c1, lane + 1, tr) <= slot));
+    if (b >= a.seqs) return;
+    cu0 = __builtin_amdgcn_readlane(c0, b);
+    cu1 = __builtin_amdgcn_readlane(c1, b);
+    len = __builtin_amdgcn_readlane(l, b);
+    base = (int64_t)__builtin_amdgcn_readlane((int)(u >> 32), b) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)u, b);
+  } else {
+    b = seq_of_slot(a, slot, tr);
+    if (b >= a.seqs) return;
+    cu0 = a.cu[b];
+    cu1 = a.cu[b + 1];
+    len = a.lens[b];
+    base = a.units[b];
+  }
+  const Seq s = seq_from(a, cu0, cu1, len);
+  const int64_t qt = slot - slot_from(a, cu0, b, tr);
   const int nq = row_tiles(a, s, tr), nt = key_tiles(a, s, tr, tk);
   if (qt < 0 || qt >= nq) return;
   const int64_t u0 = base + ((int64_t)hk * nq + qt) * nt, g0 = u0 / each, g1 = (u0 + nt - 1) / each;
@@ -875,7 +909,10 @@ __global__ __launch_bounds__(TPB) void attn_join_kernel(const Args a, int tr, in
     float up = m;
 #pragma unroll
     for (int i = 0; i < AT; ++i) {  // workgroup gi's share of this row tile: its first one unless the tile begins inside gi's units
-      const int64_t gi = min(g + i, g1), at = (gi * 2 + (u0 < gi * each ? 0 : 1)) * tr + row;
+      const int64_t gi = g + i, at = (gi * 2 + (u0 < gi * each ? 0 : 1)) * tr + row;
+      x[i] = make_float2(-INFINITY, 0.f);
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (gi > g1) continue;
       x[i] = *reinterpret_cast<const float2*>(ml + at * 2);
       v[i] = *reinterpret_cast<const float4*>(a.part + at * D + d4 * 4);
     }
@@ -886,8 +923,7 @@ __global__ __launch_bounds__(TPB) void attn_join_kernel(const Args a, int tr, in
     o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
-      const float f = g + i > g1 || x[i].x == -INFINITY ? 0.f : fast_exp2(x[i].x - up);
-      if (g + i > g1) continue;
+      const float f = x[i].x == -INFINITY ? 0.f : fast_exp2(x[i].x - up);
       l = __builtin_fmaf(x[i].y, f, l);
       o.x = __builtin_fmaf(v[i].x, f, o.x); o.y = __builtin_fmaf(v[i].y, f, o.y);
       o.z = __builtin_fmaf(v[i].z, f, o.z); o.w = __builtin_fmaf(v[i].w, f, o.w);
@@ -965,7 +1001,7 @@ int launch(hipStream_t st, const Args& a, const Plan& r) {
     hipLaunchKernelGGL((attn_many_kernel<T, D, F8, ALIGNED>), grid, dim3(TPB), lds, st, a, (int)r.split);
   }
   HMA_CHECK_LAUNCH();
-  if (r.split && r.slots > 0) {  // (no sequences: none)
+  if (r.split && a.seqs > 0) {
     const int most = (int)std::min<int64_t>(r.tr, a.tokens * a.group), per = TPB / (D / 4);
     hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3((unsigned)(r.slots * a.hk), (unsigned)((most + per - 1) / per)), dim3(TPB), 0, st, a, r.tr, r.tk);
     HMA_CHECK_LAUNCH();
