@@ -629,10 +629,11 @@ int hma_qk_rope_bwd(void* stream, const hma_qk_rope_t* p);
 /* Appends keys and values to a paged cache: row i of sequence b (rows cu[b] .. cu[b + 1], cu int32 [seqs + 1] from 0) goes to place
  * lens[b] - (cu[b + 1] - cu[b]) + i of that sequence, i.e. lens (int32 [seqs]) counts the cached tokens WITH the new ones; place p is row
  * p % page of page table[b][p / page].  k normed and rotated (r; positions NULL: the place), v as it is; both rounded once, to the
- * rows' type or (cache_e4m3) to e4m3 after division by k_scale / v_scale [hk].  q (NULL = none): normed and rotated into q_out
+ * rows' type or (cache_e4m3) to e4m3 after division by k_scale / v_scale [hk] (positive), clamped to +-448.  q (NULL = none): normed and rotated into q_out
  * [tokens][hq][d].  Cache strides in elements, the values of a row contiguous, rows 16-byte (e4m3: 8-byte) aligned.  A row whose place is negative, behind the
  * table, or in a page outside 0 .. pages - 1 is not stored.  Rows behind the last sequence (tokens > cu[seqs]) are not stored, their
- * q_out is left or (zero_tail) cleared.  r.dtype: HMA_BF16 or HMA_F16. */
+ * q_out is left or (zero_tail) cleared.  r.dtype: HMA_BF16 or HMA_F16.  q_out may be q where that is contiguous.  A place that a call writes
+ * twice (a page of two sequences) holds one of the two rows. */
 typedef struct {
   hma_rope_t r;
   int64_t tokens; int32_t hq, hk;
@@ -651,7 +652,8 @@ int hma_kv_append(void* stream, const hma_kv_append_t* p);
  * [tokens][hq] or NULL.  Row i of sequence b is at place p = lens[b] - (cu[b + 1] - cu[b]) + i and sees the keys 0 .. p (causal), the
  * last `window` of them (window > 0), or all of its sequence's lens[b] (not causal); keys in pages outside 0 .. pages - 1, or behind the table, are
  * not seen.  o = softmax(scale q k) v, lse = log sum exp; a row that sees no key: o = 0, lse = -inf.  Cache rows that no row of
- * a tile of rows sees are not read into any product, whatever they hold.  Rows behind the last sequence are left or (zero_tail) o = 0, lse = -inf.
+ * a tile of rows (32 or 128 of a sequence's tokens x shared heads) sees are not read into any product, whatever they hold; a value row that is
+ * no number and that some row of a tile sees may reach all of its tile, as 0 x NaN does in the formula.  Rows behind the last sequence are left or (zero_tail) o = 0, lse = -inf.
  * scale > 0; seqs <= 4096; cache strides in elements, rows 16-byte aligned.  ws: 16-byte aligned scratch of hma_attn_paged_ws bytes (from
  * the same struct; pointers are not looked at), one for each call in flight.  No atomics: the same bits every time. */
 typedef struct {

@@ -396,3 +396,15 @@ def test_append_custom_op_and_graph():
         q2 = ops.kv_append(s["k"], s["v"], k2, v2, table, cu, kv, q=s["q"], freqs=s["freqs"], norm="rms", q_weight=s["q_weight"], k_weight=s["k_weight"])
         torch.cuda.synchronize()
         assert torch.equal(out, q2) and torch.equal(kc, k2) and torch.equal(vc, v2)
+
+
+def test_append_in_place():
+    """q_out may be q: every row is read before the wave that read it writes it."""
+    g = gen(50)
+    new, lens = [700, 1, 40], [700, 90, 400]
+    table, cu, kv, kc, vc, tokens = paged(new, lens, 16, 2, 64, BF, g)
+    s = make(tokens, 12, 2, 64, 64, "rms", BF, seed=51)
+    kw = dict(freqs=s["freqs"], norm="rms", q_weight=s["q_weight"], k_weight=s["k_weight"])
+    want = ops.kv_append(s["k"], s["v"], kc, vc, table, cu, kv, q=s["q"], **kw)
+    q = s["q"].contiguous()
+    assert ops.kv_append(s["k"], s["v"], kc, vc, table, cu, kv, q=q, q_out=q, **kw) is q and torch.equal(q, want)
