@@ -18,8 +18,9 @@
 // Reductions: everything in 32 bits; each output is rounded once.
 // Measured (bf16): forward of 81920 tokens x 16 heads of 32, three axes, layer norm: 40 us = 4.2 TB/s of 168 MB; of 8191 x 40 heads of 128,
 // RMS norm: 34 us = 4.9 TB/s.  7 tokens x 40 heads of 128: 4.9 us, a launch and one trip to memory.  The cache form: 8 frames of 320 tokens x 32
-// rows of 32: 12 us; 7.9 thousand tokens x 16 rows of 128 into e4m3: 21 us = 2.3 TB/s (four dependent loads stand in front of a wave's
-// first store -- sequence, length, page, row -- and a wave has two or three tokens); one token of 64 sequences x 48 rows of 128: 7.4 us.
+// rows of 32: 12 us; 7.9 thousand tokens x 16 rows of 128 into e4m3: 21 us = 2.3 TB/s (what a wave does once, and four dependent loads in front
+// of its first store -- sequence, length, page, row -- for two tokens); 128 thousand such tokens: 250 us = 3.1 TB/s, into bf16 224 us =
+// 4.7 TB/s; one token of 64 sequences x 48 rows of 128: 7.4 us.
 #include "hma_common.h"
 #include "../../include/hma_hip.h"
 
@@ -90,7 +91,7 @@ template <> struct Io<float> {
 };
 
 // 8 values -> 8 e4m3 bytes, nearest even, clamped to the type's largest value (a NaN stays one)
-__device__ __forceinline__ float sat8(float x) { return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.f, 448.f); }
+__device__ __forceinline__ float sat8(float x) { return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 448.f), -448.f); }
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f, float mul) {
   uint2 w;
   int a = 0, b = 0;
@@ -333,7 +334,7 @@ struct Part {
 };
 
 template <typename T, bool APPEND, bool F8, int NORM, bool INTER>
-__global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_fwd_kernel(const FwdArgs g) {
+__global__ __launch_bounds__(TPB, (APPEND && NORM != HMA_NORM_NONE) || Io<T>::SIZE == 4 ? 3 : 4) void rope_fwd_kernel(const FwdArgs g) {
   constexpr int U = 2, SZ = Io<T>::SIZE, CS = F8 ? 1 : SZ;  // units in flight, bytes of a value and of a cached one
   __shared__ Lds L;
   const Shape& a = g.s;
@@ -348,13 +349,14 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
   const int er = in_row ? e0 : 0, hqk = a.hq + a.hk, heads = hqk + (APPEND ? a.hk : 0);
   const float inv_d = 1.0f / (float)a.d;
   const bool places = APPEND && !a.positions;
+  const int64_t k_lane = APPEND ? (sub * g.kc_head + e0) * CS : 0, v_lane = APPEND ? (sub * g.vc_head + e0) * CS : 0;  // this lane's part of a cache address
   Part pq, pk, pv;
   pq.begin(g.q, g.q_tok, g.q_head, SZ, sub, er);
   pk.begin(g.k, g.k_tok, g.k_head, SZ, sub, er);
   if (APPEND) pv.begin(g.v, g.v_tok, g.v_head, SZ, sub, er);
 
-  // the next U units from (token t of batch bt, group p) on; a unit behind the batch's last is loaded as that one
-  auto fetch = [&](int64_t bt, int t, int p, typename Io<T>::raw* r) {
+  // the next U units from (token t of batch bt, group p) on, with their heads' scales; a unit behind the batch's last is loaded as that one
+  auto fetch = [&](int64_t bt, int t, int p, typename Io<T>::raw* r, float* scale) {
     const int64_t tok0 = bt * a.wt;
     const int nt = (int)min((int64_t)a.wt, a.tokens - tok0);
 #pragma unroll
@@ -366,6 +368,7 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
       if (APPEND && h >= hqk) at = pv.of(tok, h0 - hqk) + pv.lane;
       if (h >= heads) at = pk.of(tok, 0) + er * SZ;
       r[i] = Io<T>::load(at);
+      if (F8) scale[i] = h >= hqk && h < heads ? g.v_scale[h - hqk] : g.k_scale[h >= a.hq && h < hqk ? h - a.hq : 0];
       if (++p == np) {
         if (t + 1 < nt) p = 0, ++t; else p = np - 1;
       }
@@ -373,12 +376,13 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
   };
   const bool mine = np > 0 && batch < a.batches;
   typename Io<T>::raw nx[U];
+  float ns[U];
   double pos[2] = {0.0, 0.0};
   Angles an;
   const int st = APPEND ? max((g.seqs + 63) >> 6, 1) : 1;
   int sample = 0x7fffffff;
   if (mine) {
-    fetch(batch, 0, 0, nx);
+    fetch(batch, 0, 0, nx, ns);
     if (APPEND && (lane + 1) * st <= g.seqs) sample = g.cu[(lane + 1) * st];
     an.begin(a, lane);
     if (!places) an.position(a, batch * a.wt, pos);
@@ -409,15 +413,19 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
     int t_cur = -1;
     for (int t = 0, p = 0; t < nt;) {
       typename Io<T>::raw r[U];
+      float inv[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) r[i] = nx[i];
+      for (int i = 0; i < U; ++i) {
+        r[i] = nx[i];
+        if (F8) inv[i] = __builtin_amdgcn_rcpf(ns[i]);  // (one step of 32 bits off at most)
+      }
       {
         int t2 = t, p2 = p + U;
         while (p2 >= np && t2 < nt) p2 -= np, ++t2;
         if (t2 < nt)
-          fetch(batch, t2, p2, nx);
+          fetch(batch, t2, p2, nx, ns);
         else if (nb < a.batches)
-          fetch(nb, 0, 0, nx);
+          fetch(nb, 0, 0, nx, ns);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -438,7 +446,7 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
             read8(&L.w[!is_q][1][er], b);
           }
         }
-        float x[8], y[8], n[8];
+        float x[8], y[8] = {}, n[8];
         Io<T>::unpack(r[i], x);
         if (!APPEND || h0 < hqk) {  // (a group of values alone has neither norm nor rotation)
           if (NORM != HMA_NORM_NONE) {
@@ -457,20 +465,20 @@ __global__ __launch_bounds__(TPB, APPEND || Io<T>::SIZE == 4 ? 3 : 4) void rope_
           if (live) Io<T>::store(dst, y);
         } else {
           const int off = __builtin_amdgcn_readfirstlane(W.off[t]), page = __builtin_amdgcn_readfirstlane(W.page[t]);
-          if (is_v) {
+          if (h0 + a.hp > hqk) {  // some of the group's rows are values
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[e];
+            for (int e = 0; e < 8; ++e) y[e] = is_v ? x[e] : y[e];
           }
-          if (is_q && off == -2) {
+          if (off == -2) {  // (nothing but zeros is stored of it)
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = 0.f;
           }
           if (live && is_q && (off != -2 || g.zero_tail)) Io<T>::store((uint8_t*)g.q_out + (tok * a.hq + h0) * a.d * SZ + (sub * a.d + e0) * SZ, y);
           if (live && !is_q && off >= 0) {
             const int64_t ks = page * g.kc_page + off * g.kc_tok + (h0 - a.hq) * g.kc_head, vs = page * g.vc_page + off * g.vc_tok + (h0 - hqk) * g.vc_head;
-            uint8_t* dst = is_v ? (uint8_t*)g.vc + (vs + sub * g.vc_head + e0) * CS : (uint8_t*)g.kc + (ks + sub * g.kc_head + e0) * CS;
+            uint8_t* dst = is_v ? (uint8_t*)g.vc + vs * CS + v_lane : (uint8_t*)g.kc + ks * CS + k_lane;
             if (F8)
-              store_e4m3(dst, y, 1.0f / (is_v ? g.v_scale[h - hqk] : g.k_scale[h - a.hq]));
+              store_e4m3(dst, y, inv[i]);
             else
               Io<T>::store(dst, y);
           }
@@ -677,10 +685,10 @@ __global__ __launch_bounds__(1024) void rope_wsum_kernel(const float* part, int 
 }
 
 // Workgroups of a forward launch: a wave per (batch, share of the heads), at most what is resident (4 a compute unit, 3 with the cache's
-// addresses); a wave then walks several batches.  With a third more than resident the last quarter of a launch runs on a third of the
+// addresses and a norm); a wave then walks several batches.  With a third more than resident the last quarter of a launch runs on a third of the
 // chip: the backward of 81920 x 16 heads of 32 took 87 us instead of 68.
 unsigned fwd_groups(const Shape& s, bool append) {
-  const int64_t want = (s.batches * s.py + WAVES - 1) / WAVES, most = 256 * (append ? 3 : 4);
+  const int64_t want = (s.batches * s.py + WAVES - 1) / WAVES, most = 256 * (append && s.norm != HMA_NORM_NONE ? 3 : 4);
   return (unsigned)(want < most || s.py > 1 ? want : most);
 }
 template <typename T, bool APPEND, bool F8, int NORM>
