@@ -408,3 +408,28 @@ def test_append_in_place():
     want = ops.kv_append(s["k"], s["v"], kc, vc, table, cu, kv, q=s["q"], **kw)
     q = s["q"].contiguous()
     assert ops.kv_append(s["k"], s["v"], kc, vc, table, cu, kv, q=q, q_out=q, **kw) is q and torch.equal(q, want)
+
+
+def test_append_what_is_no_number_into_e4m3():
+    """Beyond the type's largest value: that value; a NaN stays one; the others of the row are as without."""
+    g = gen(60)
+    table, cu, kv, kc, vc, tokens = paged([5, 2], [5, 30], 16, 2, 64, BF, g)
+    s = make(tokens, 2, 2, 64, 0, "none", BF, seed=61)
+    scales = dict(k_scale=torch.full((2,), 0.02, device=DEV), v_scale=torch.full((2,), 0.03, device=DEV))
+    k, v = s["k"].clone(), s["v"].clone()
+    for x in (k, v):
+        x[0, 0, 3], x[1, 1, 63], x[5, 0, 0], x[6, 1, 8] = float("inf"), -float("inf"), float("nan"), 1e4
+    got = []
+    for a, b in ((s["k"], s["v"]), (k, v)):
+        c = torch.zeros_like(kc).to(F8), torch.zeros_like(vc).to(F8)
+        ops.kv_append(a, b, *c, table, cu, kv, **scales)
+        got.append(c)
+    place = [0, 1, 2, 3, 4, 28, 29]
+    seq = [0] * 5 + [1] * 2
+    pg = table[seq, [p // 16 for p in place]].long()
+    off = torch.tensor(place, device=DEV) % 16
+    for clean, odd, x, y in zip(*got, (k, v), (s["k"], s["v"])):
+        a, b = clean[pg, :, off].float(), odd[pg, :, off].float()
+        same = x.float() == y.float()
+        assert int((~same).sum()) == 4 and torch.equal(a[same], b[same])
+        assert b[0, 0, 3] == 448 and b[1, 1, 63] == -448 and b[5, 0, 0].isnan() and b[6, 1, 8] == 448
