@@ -353,3 +353,22 @@ def test_rollout():
                     rms = float((o[at:at + news[b], h].double() - ref).norm() / ref.norm())
                     assert rms < 2e-2, (step, b, h, rms)  # what independent roundings of that size leave of the bound
             at += news[b]
+
+
+@pytest.mark.parametrize("hq,new,lens", [(64, [1, 3], [70, 300]), (160, [2, 1, 9], [40, 130, 9]), (160, [1], [1])])
+def test_groups_larger_than_a_tile_of_rows(hq, new, lens):
+    for window in (0, 20):
+        s = batch(new, lens, 16, hq, 1, 64, BF, seed=30, tail=1)
+        check(s, call(s, 0.125, True, window), 0.125, True, window)
+
+
+def test_the_most_sequences():
+    lens = [(13 * i) % 70 for i in range(4096)]
+    s = batch([1] * 4096, lens, 16, 1, 1, 64, HF, seed=31)
+    got = call(s, 0.125)
+    for lo in (0, 2040, 4090):  # against calls of six sequences each
+        part = dict(s, q=s["q"][lo:lo + 6], table=s["table"][lo:lo + 6], lens=s["lens"][lo:lo + 6], cu=torch.arange(7, dtype=torch.int32, device=DEV),
+                    new=[1] * 6, lengths=lens[lo:lo + 6])
+        check(part, (got[0][lo:lo + 6], got[1][lo:lo + 6]), 0.125, True, 0)
+    with pytest.raises(RuntimeError):
+        call(batch([1] * 4097, [1] * 4097, 16, 1, 1, 64, HF), 0.125)
