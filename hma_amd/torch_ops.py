@@ -409,8 +409,16 @@ def _(dy_q, dy_k, q, k, freqs, positions, axes, interleaved, amplitude, norm, q_
     return [q.new_empty(q.shape), k.new_empty(k.shape)] + [torch.empty_like(w) for w in (q_weight, q_bias, k_weight, k_bias) if w is not None]
 
 
-def _plain(t: torch.Tensor) -> bool:
-    return type(t) is torch.Tensor or type(t) is torch.nn.Parameter
+def _plain(*ts) -> bool:
+    """Whether nothing stands between the autograd formula and the kernels: no dispatch mode is on (a tracer, a counter, a checkpointing
+    policy), and every tensor is one whose memory holds its values (no subclass, no functional wrapper, no negated view).  Only then may
+    the launch be called by itself, which saves the dispatcher's second round; everything else goes through torch.ops."""
+    if torch._C._len_torch_dispatch_stack():
+        return False
+    for t in ts:
+        if t is not None and ((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or t.is_neg() or torch._is_functional_tensor(t)):
+            return False
+    return True
 
 
 class _QkRope(torch.autograd.Function):
@@ -419,9 +427,9 @@ class _QkRope(torch.autograd.Function):
         q, k, freqs, positions, axes, interleaved, amplitude, norm, qw, qb, kw, kb, eps = a
         ctx.save_for_backward(q, k, freqs, positions, axes, qw, qb, kw, kb)
         ctx.args = (interleaved, amplitude, norm, eps)
-        if _plain(q):
+        if _plain(q, k, freqs, positions, axes, qw, qb, kw, kb):
             return _qk_rope(*a)
-        with torch._C._AutoDispatchBelowAutograd():  # tracing tensors take the dispatcher to the shapes above
+        with torch._C._AutoDispatchBelowAutograd():
             return torch.ops.hma.qk_rope(*a)
 
     @staticmethod
@@ -429,7 +437,7 @@ class _QkRope(torch.autograd.Function):
     def backward(ctx, dy_q, dy_k):
         q, k, freqs, positions, axes, *w = ctx.saved_tensors
         interleaved, amplitude, norm, eps = ctx.args
-        fn = _qk_rope_bwd if _plain(q) else torch.ops.hma.qk_rope_bwd
+        fn = _qk_rope_bwd if _plain(dy_q, dy_k, q, k, freqs, positions, axes, *w) else torch.ops.hma.qk_rope_bwd
         d = iter(fn(dy_q, dy_k, q, k, freqs, positions, axes, interleaved, amplitude, norm, *w, eps))
         return (next(d), next(d), None, None, None, None, None, None, *(None if x is None else next(d) for x in w), None)
 

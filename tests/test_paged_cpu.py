@@ -7,6 +7,8 @@ import math
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import hma_amd.torch_ops as T
 from hma_amd import _lib, ops
@@ -247,6 +249,80 @@ def test_fake_shapes():
         assert out.shape == q.shape
         o, lse = torch.ops.hma.attn_paged(q, kc, kc, tab, cu, lens, 0.2, True, 0, None, None)
         assert o.shape == q.shape and lse.shape == (5, 4) and lse.dtype == F32
+
+
+@pytest.fixture
+def on_the_host(monkeypatch):
+    """qk_rope and its backward registered for host tensors with a stand-in for the launches: x 3 + w, and gradients of their own shapes."""
+    def fwd(q, k, freqs, positions, *, q_weight=None, k_weight=None, **kw):
+        return tuple(t * 3 + (0 if w is None else w.to(t.dtype)) for t, w in ((q, q_weight), (k, k_weight)))
+
+    def bwd(dy_q, dy_k, q, k, freqs, positions, *, q_weight=None, k_weight=None, **kw):
+        return (dy_q * 3, dy_k * 3, *(None if w is None else d.to(w.dtype).sum((0, 1)) for d, w in ((dy_q, q_weight), (dy_q, None), (dy_k, k_weight), (dy_k, None))))
+
+    monkeypatch.setattr(ops, "qk_rope_fwd", fwd)
+    monkeypatch.setattr(ops, "qk_rope_bwd", bwd)
+    lib = torch.library.Library("hma", "IMPL")
+    lib.impl("qk_rope", T._qk_rope, "CPU")
+    lib.impl("qk_rope_bwd", T._qk_rope_bwd, "CPU")
+    lib.impl("qk_rope", lambda *a: T._QkRope.apply(*a), "AutogradCPU")
+    yield
+    lib._destroy()
+
+
+def rope_and_gradients(q, k, w):
+    f, pos = torch.ones(8, dtype=torch.float64), torch.arange(5)
+    leaves = [t.detach().requires_grad_() for t in (q, k, w)]
+    y = torch.ops.hma.qk_rope(leaves[0], leaves[1], f, pos, None, False, 1.0, "rms", leaves[2], None, leaves[2], None, 1e-5)
+    return [t.detach() for t in y] + list(torch.autograd.grad(y, leaves, [y[0].detach() * 2, y[1].detach()]))
+
+
+def rope_inputs(seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(*s, generator=g) for s in ((5, 4, 32), (5, 2, 32), (32,))]
+
+
+@pytest.mark.parametrize("mode", ["real", "fake"])
+def test_traced_graphs_hold_the_op_and_its_backward(on_the_host, mode):
+    graph = make_fx(rope_and_gradients, tracing_mode=mode)(*rope_inputs(0))
+    called = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    assert called.count(torch.ops.hma.qk_rope.default) == 1 and called.count(torch.ops.hma.qk_rope_bwd.default) == 1
+    for seed in (0, 1):  # the inputs of the trace and others
+        got, want = graph(*rope_inputs(seed)), rope_and_gradients(*rope_inputs(seed))
+        assert len(got) == len(want) == 5 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_dispatch_modes_see_the_op_and_its_backward(on_the_host):
+    seen = []
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func)
+            return func(*args, **(kwargs or {}))
+
+    with Record():
+        got = rope_and_gradients(*rope_inputs(2))
+    assert seen.count(torch.ops.hma.qk_rope.default) == 1 and seen.count(torch.ops.hma.qk_rope_bwd.default) == 1
+    assert all(torch.equal(a, b) for a, b in zip(got, rope_and_gradients(*rope_inputs(2))))
+
+
+def test_negated_views_are_resolved(on_the_host, monkeypatch):
+    """A view whose values are the negatives of its memory reaches the kernels as the values, in whichever place it is given."""
+    fwd, bwd = ops.qk_rope_fwd, ops.qk_rope_bwd
+
+    def plain(fn):
+        def f(*a, **kw):
+            assert not any(t.is_neg() for t in (*a, *kw.values()) if isinstance(t, torch.Tensor))
+            return fn(*a, **kw)
+        return f
+
+    monkeypatch.setattr(ops, "qk_rope_fwd", plain(fwd))
+    monkeypatch.setattr(ops, "qk_rope_bwd", plain(bwd))
+    q, k, w = rope_inputs(3)
+    for i in range(3):
+        a, b = [q, k, w], [q, k, w]
+        a[i], b[i] = torch._neg_view(a[i]), -b[i]
+        assert all(torch.equal(x, y) for x, y in zip(rope_and_gradients(*a), rope_and_gradients(*b)))
 
 
 def test_frequencies():
