@@ -564,7 +564,7 @@ def attn_paged_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         q_tok, q_head, _ = q.stride()
         p, n = AttnPaged(), C.c_int64()
         _ATTN_PAGED.pack_into(p, 0, q.data_ptr(), out.data_ptr(), lse.data_ptr(), *lists, 0, 0, tokens, q_tok, q_head, *strides, table_stride, hq, cache[1], d,
-                              _DTYPE[kind], *sizes, causal, window, zero_tail, scale, 0)
+                              _DTYPE[kind], *sizes, causal, min(window, 0x7fffffff), zero_tail, scale, 0)  # (lengths are below 2^31)
         _lib.call("hma_attn_paged_ws", C.byref(p), C.byref(n))
         if n.value:
             ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)

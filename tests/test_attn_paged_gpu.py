@@ -372,3 +372,12 @@ def test_the_most_sequences():
         check(part, (got[0][lo:lo + 6], got[1][lo:lo + 6]), 0.125, True, 0)
     with pytest.raises(RuntimeError):
         call(batch([1] * 4097, [1] * 4097, 16, 1, 1, 64, HF), 0.125)
+
+
+def test_windows_beyond_every_length():
+    for new, lens in (([1, 3], [700, 90]), ([200, 70], [500, 70])):
+        s = batch(new, lens, 16, 4, 2, 64, BF, seed=42)
+        want = call(s, 0.125)
+        for window in (10 ** 6, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+            got = call(s, 0.125, True, window)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), window

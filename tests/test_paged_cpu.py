@@ -135,6 +135,17 @@ def test_the_good_calls_launch(host):
         ops.attn_paged_fwd(torch.zeros(3, 4, 48, dtype=BF), *(torch.zeros(4, 2, 16, 48, dtype=BF),) * 2, *list(a.values())[2:], 0.2)
 
 
+def test_windows_of_any_size_launch(host, monkeypatch):
+    """A window larger than a 32-bit number is one that no sequence reaches, not an error of the argument structure."""
+    a, _ = cache_args()
+    del a["k"], a["v"]
+    passed = []
+    monkeypatch.setattr(ops._lib, "call", lambda name, *p: passed.append((name, [x._obj for x in p if hasattr(x, "_obj")][0])))
+    for window in (0, 5, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1, 2 ** 70):
+        ops.attn_paged_fwd(torch.zeros(3, 4, 32, dtype=BF), *a.values(), 0.2, window=window)
+        assert passed[-1][0] == "hma_attn_paged_fwd" and passed[-1][1].window == min(window, 2 ** 31 - 1)
+
+
 def test_host_tensors_are_refused():
     a, kw = rope_args()
     with pytest.raises(RuntimeError):
