@@ -90,15 +90,25 @@ template <> struct Io<float> {
   static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((float*)p)[i] = v; }
 };
 
-// 8 values -> 8 e4m3 bytes, nearest even, clamped to the type's largest value (a NaN stays one)
-__device__ __forceinline__ float sat8(float x) { return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 448.f), -448.f); }
-__device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f, float mul) {
+// 8 values -> 8 e4m3 bytes of x / scale: nearest even, clamped to the type's largest value (a NaN stays one).  The product with the hardware's
+// reciprocal (one step off) alone lands on the wrong side of a border between two e4m3 values where the quotient lies on it or next to it
+// (an odd multiple of a power of two for a scale: one value in twenty thousand); its remainder q scale - x, exact in one fma, puts that
+// right.  128 thousand tokens x 16 rows: 250 -> 252 us, with the compiler's division 311.  x is clamped, not q: an infinity has no remainder.
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f, float scale) {
+  const float inv = __builtin_amdgcn_rcpf(scale), lim = fminf(448.f * scale, 3.4e38f);
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = __builtin_elementwise_maximum(__builtin_elementwise_minimum(f[e], lim), -lim);
+    q[e] = x * inv;
+    q[e] = __builtin_fmaf(-__builtin_fmaf(q[e], scale, -x), inv, q[e]);  // (in this order a zero keeps its sign)
+  }
   uint2 w;
   int a = 0, b = 0;
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[0] * mul), sat8(f[1] * mul), a, false);
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[2] * mul), sat8(f[3] * mul), a, true);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[4] * mul), sat8(f[5] * mul), b, false);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(sat8(f[6] * mul), sat8(f[7] * mul), b, true);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], b, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
   w.x = (uint32_t)a;
   w.y = (uint32_t)b;
   *reinterpret_cast<uint2*>(p) = w;
@@ -413,11 +423,11 @@ __global__ __launch_bounds__(TPB, (APPEND && NORM != HMA_NORM_NONE) || Io<T>::SI
     int t_cur = -1;
     for (int t = 0, p = 0; t < nt;) {
       typename Io<T>::raw r[U];
-      float inv[U];
+      float scale[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         r[i] = nx[i];
-        if (F8) inv[i] = __builtin_amdgcn_rcpf(ns[i]);  // (one step of 32 bits off at most)
+        if (F8) scale[i] = ns[i];
       }
       {
         int t2 = t, p2 = p + U;
@@ -478,7 +488,7 @@ __global__ __launch_bounds__(TPB, (APPEND && NORM != HMA_NORM_NONE) || Io<T>::SI
             const int64_t ks = page * g.kc_page + off * g.kc_tok + (h0 - a.hq) * g.kc_head, vs = page * g.vc_page + off * g.vc_tok + (h0 - hqk) * g.vc_head;
             uint8_t* dst = is_v ? (uint8_t*)g.vc + vs * CS + v_lane : (uint8_t*)g.kc + ks * CS + k_lane;
             if (F8)
-              store_e4m3(dst, y, inv[i]);
+              store_e4m3(dst, y, scale[i]);
             else
               Io<T>::store(dst, y);
           }

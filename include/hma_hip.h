@@ -629,7 +629,7 @@ int hma_qk_rope_bwd(void* stream, const hma_qk_rope_t* p);
 /* Appends keys and values to a paged cache: row i of sequence b (rows cu[b] .. cu[b + 1], cu int32 [seqs + 1] from 0) goes to place
  * lens[b] - (cu[b + 1] - cu[b]) + i of that sequence, i.e. lens (int32 [seqs]) counts the cached tokens WITH the new ones; place p is row
  * p % page of page table[b][p / page].  k normed and rotated (r; positions NULL: the place), v as it is; both rounded once, to the
- * rows' type or (cache_e4m3) to e4m3 after division by k_scale / v_scale [hk] (positive), clamped to +-448.  q (NULL = none): normed and rotated into q_out
+ * rows' type or (cache_e4m3) to e4m3 after division (in 32 bits) by k_scale / v_scale [hk] (from 2^-100 to 2^100), clamped to +-448.  q (NULL = none): normed and rotated into q_out
  * [tokens][hq][d].  Cache strides in elements, the values of a row contiguous, rows 16-byte (e4m3: 8-byte) aligned.  A row whose place is negative, behind the
  * table, or in a page outside 0 .. pages - 1 is not stored.  Rows behind the last sequence (tokens > cu[seqs]) are not stored, their
  * q_out is left or (zero_tail) cleared.  r.dtype: HMA_BF16 or HMA_F16.  q_out may be q where that is contiguous.  A place that a call writes

@@ -433,3 +433,23 @@ def test_append_what_is_no_number_into_e4m3():
         same = x.float() == y.float()
         assert int((~same).sum()) == 4 and torch.equal(a[same], b[same])
         assert b[0, 0, 3] == 448 and b[1, 1, 63] == -448 and b[5, 0, 0].isnan() and b[6, 1, 8] == 448
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_rounds_the_quotient(dtype):
+    """What goes into an e4m3 cache is x / scale in 32 bits, rounded: every finite value of the rows' type, against scales whose quotients
+    lie on the borders between two e4m3 values (odd multiples of powers of two) and others; exact, zeros' signs too."""
+    g = torch.Generator().manual_seed(70)
+    scales = torch.cat([(2 * torch.arange(32) + 1) * 2.0 ** -11, 0.001 + 0.02 * torch.rand(28, generator=g), torch.tensor([1.0, 448.0, 3e-20, 5e15])]).float()
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = torch.where(x.isnan(), torch.zeros_like(x), x).view(512, 1, 128).expand(512, 64, 128)
+    page = 64
+    kc, vc = (torch.zeros(8, 64, page, 128, dtype=F8, device=DEV) for _ in range(2))
+    table = torch.arange(8, dtype=torch.int32, device=DEV)[None]
+    cu, lens = torch.tensor([0, 512], dtype=torch.int32, device=DEV), torch.tensor([512], dtype=torch.int32, device=DEV)
+    ops.kv_append(x.to(DEV), x.flip(1).to(DEV), kc, vc, table, cu, lens, k_scale=scales.to(DEV), v_scale=scales.flip(0).to(DEV))
+    for cache, s in ((kc, scales), (vc, scales.flip(0))):
+        got = cache.transpose(1, 2).reshape(512, 64, 128).cpu()
+        want = (x.float() / s[:, None]).clamp(-448, 448).to(F8)
+        off = got.view(torch.uint8) != want.view(torch.uint8)
+        assert not off.any(), (int(off.sum()), s[off.any(0).any(-1)].tolist(), x[off][:4].tolist(), got[off][:4].float().tolist(), want[off][:4].float().tolist())
