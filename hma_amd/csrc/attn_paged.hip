@@ -9,9 +9,10 @@
 // Products.  S^T = K Q^T by v_mfma_f32_32x32x16: a lane then holds ONE row and 16 of 32 keys, the softmax is in-lane with one exchange
 // between the half-waves, and the packed probabilities are the B operand of O^T = V^T P^T as they lie (the contraction index is permuted
 // alike on both sides); V^T comes out of row-major LDS by transposing reads.  Scores, maxima, sums and O in 32 bits; probabilities are
-// rounded once to the rows' 16-bit type for the second product (2^-9 or 2^-12 relative, below what the output's own rounding does), the
-// sums take them unrounded.  The running maximum is raised only when a row exceeds it by 2^8: probabilities then reach 256 instead of 1,
-// which changes no relative rounding, and O is rescaled a few times instead of at every step.
+// rounded once to the rows' 16-bit type for the second product, as the matrix instruction wants both operands of one type (2^-8 or 2^-11
+// relative each, about as much as the output's own rounding adds: the error against 64 bits is 1.2 to 1.4 times that of a softmax in 32
+// bits); the sums take them unrounded.  The running maximum is raised only when a row exceeds it by far (Range): that changes no relative
+// rounding, and O is rescaled a few times instead of at every step.
 // Pages.  A lane looks up the page of one key, the loads take it by a lane exchange.  A key outside what the tile sees, or in a page
 // outside the cache, is loaded as zeros, so nothing that is not a sequence's own reaches a product.  e4m3 caches are widened to the rows'
 // type (exactly) on their way into LDS; the scales join the scores' factor and the output's.
@@ -36,7 +37,6 @@ typedef short v8s16_t __attribute__((ext_vector_type(8)));
 
 constexpr int TPB = 256, WAVES = 4;
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr float LAZY = 8.0f;  // how far (in powers of two) a row may exceed its running maximum before O is rescaled
 constexpr int PAD = 16;       // few rows: LDS rows of D + 16 values (two-way conflicts of the transposing reads, which do not bound that kernel)
 
 struct Args {
@@ -55,6 +55,18 @@ struct Args {
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Probabilities are 2^(score - m), m = running maximum - LIFT; a row may exceed that maximum by LAZY powers of two before O is rescaled.  fp16 has
+// 15 binades above 1 and, at full precision, 14 below: with the largest probability at 2^10 one keeps all its bits down to 2^-24 of it and is lost only
+// below 2^-35 (at 1 it would be from 2^-25 on, and 131072 keys 17 powers of e behind one with a value of zero came out 20 % off).  bf16 has the
+// range of 32 bits.  SUM: what no 16 probabilities together may exceed, so that none is over 2^LAZY or what the type holds.
+template <typename T> struct Range;
+template <> struct Range<__bf16> {
+  static constexpr float LIFT = 0.f, LAZY = 8.f, SUM = 16.f * 256.f;
+};
+template <> struct Range<_Float16> {
+  static constexpr float LIFT = 10.f, LAZY = 5.f, SUM = 65504.f;
+};
 
 template <typename T> struct Op;  // T: __bf16 or _Float16
 template <> struct Op<__bf16> {
@@ -181,7 +193,7 @@ template <typename T, int D>
 struct Rows {
   uint4 q[D / 16];
   f32x16_t o[D / 32];
-  float m, l;       // running maximum (powers of two), sum of this half-wave's keys
+  float m, l;       // running maximum less LIFT (powers of two), sum of this half-wave's keys
   int32_t lo, hi;   // keys that the row sees
   bool live;
   int64_t at;       // its row of o (tokens x heads)
@@ -241,7 +253,7 @@ struct Rows {
       for (int e = 0; e < 16; ++e) s[k][e] = w & (1u << (8 * (e >> 2) + (e & 3))) ? -INFINITY : s[k][e];
     }
   }
-  // the largest score of a row's KB blocks in powers of two (c: the scores' factor)
+  // the largest score of a row's KB blocks in powers of two less LIFT (c: the scores' factor)
   template <int KB>
   __device__ __forceinline__ float largest(const f32x16_t (&s)[KB], float c) const {
     float x0 = -INFINITY, x1 = -INFINITY;
@@ -254,11 +266,11 @@ struct Rows {
       }
     const uint32_t x = __float_as_uint(fmaxf(x0, x1));
     const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);  // the two half-waves' values in every lane
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
+    return __builtin_fmaf(fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])), c, -Range<T>::LIFT);
   }
-  // the running maximum raised where a row exceeds it by far
-  __device__ __forceinline__ void raise(float x) {
-    if (__ballot(x > m + LAZY)) {  // also where m is still -inf
+  // the running maximum raised where a row exceeds it by far (lazy: how far, in powers of two)
+  __device__ __forceinline__ void raise(float x, float lazy) {
+    if (__ballot(x > m + lazy)) {  // also where m is still -inf
       const float up = fmaxf(m, x), f = m == -INFINITY ? 0.f : fast_exp2(m - up);
       l *= f;
 #pragma unroll
@@ -502,7 +514,7 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
         r.template scores<KB>(mine, sc);
         if (key0 < t.lo_max || key0 + KEYS > t.hi_min) r.template mask<KB>(sc, key0);
         if (bad) r.template mask_bad<KB>(sc, bad);
-        r.raise(r.template largest<KB>(sc, c));
+        r.raise(r.template largest<KB>(sc, c), Range<T>::LAZY);
 #pragma unroll
         for (int k = 0; k < KB; ++k) r.weigh(sc[k], c, p[k]);
         wave_lds_order();
@@ -786,12 +798,13 @@ __global__ __launch_bounds__(TPB, ManyWaves<D>::value) void attn_many_kernel(con
             }
             asm volatile("" : "+v"(sum));  // (here, not where the values are wanted)
           };
-          // No maximum is sought as long as no row's probabilities of a block add up to more than 16 x 2^LAZY (then none is over that, which
-          // fp16 holds) and every row has a maximum: the sum is needed anyway.  Otherwise: the maximum, and the block again.
+          // No maximum is sought as long as no row's probabilities of a block add up to more than SUM and every row has a maximum: the sum
+          // is needed anyway.  Otherwise: the maximum, and the block again (fp16, whose SUM is reached below 2^LAZY each, takes any new maximum:
+          // the next blocks would come here again).
           const auto settle_max = [&](int k) {
-            if (__ballot(!(sum <= 16.0f * 256.0f) || r.m == -INFINITY)) {
+            if (__ballot(!(sum <= Range<T>::SUM) || r.m == -INFINITY)) {
               f32x16_t one[1] = {sc[k]};
-              r.raise(r.template largest<1>(one, c));
+              r.raise(r.template largest<1>(one, c), Range<T>::LIFT > 0.f ? 0.f : Range<T>::LAZY);
               sub = r.m == -INFINITY ? 0.f : r.m;
               sum = 0.f;
               weigh(sc[k], 0, 16);

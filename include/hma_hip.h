@@ -651,7 +651,9 @@ int hma_kv_append(void* stream, const hma_kv_append_t* p);
  * HMA_BF16 or HMA_F16; hq a multiple of hk, query head h reads key head h / (hq / hk); o [tokens][hq][d] contiguous, lse fp32
  * [tokens][hq] or NULL.  Row i of sequence b is at place p = lens[b] - (cu[b + 1] - cu[b]) + i and sees the keys 0 .. p (causal), the
  * last `window` of them (window > 0), or all of its sequence's lens[b] (not causal); keys in pages outside 0 .. pages - 1, or behind the table, are
- * not seen.  o = softmax(scale q k) v, lse = log sum exp; a row that sees no key: o = 0, lse = -inf.  Cache rows that no row of
+ * not seen.  o = softmax(scale q k) v, lse = log sum exp; a row that sees no key: o = 0, lse = -inf.  Scores, sums and o are formed in 32
+ * bits; the probabilities enter the product with v in the rows' type, which moves o by about as much as its own rounding (bf16: 2^-8 of each; fp16: 2^-11
+ * of each, and what lies below 2^-24 of the row's largest is off by up to 2^-35 of that).  Cache rows that no row of
  * a tile of rows (32 or 128 of a sequence's tokens x shared heads) sees are not read into any product, whatever they hold; a value row that is
  * no number and that some row of a tile sees may reach all of its tile, as 0 x NaN does in the formula.  Rows behind the last sequence are left or (zero_tail) o = 0, lse = -inf.
  * scale > 0; seqs <= 4096; cache strides in elements, rows 16-byte aligned.  ws: 16-byte aligned scratch of hma_attn_paged_ws bytes (from

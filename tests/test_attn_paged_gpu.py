@@ -381,3 +381,56 @@ def test_windows_beyond_every_length():
         for window in (10 ** 6, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
             got = call(s, 0.125, True, window)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), window
+
+
+# (heads, key heads, sequences, new tokens of each, keys): few rows in many shares and in few, many rows split along the keys, unsplit
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("hq,hk,seqs,n,m", [(4, 1, 1, 1, 131072), (8, 8, 96, 1, 131072), (8, 8, 30, 40, 131072), (96, 96, 1, 2700, 40000)])
+@pytest.mark.parametrize("sink", ["first", "last", "inside"])
+def test_what_a_far_larger_score_leaves_of_fp16(d, hq, hk, seqs, n, m, sink):
+    """One key takes nearly all of the weight and has a value of zero: the output is what the others, up to 20 powers of e behind it, add up to.
+    All rows are alike: with w = e^-gap, o = w sum v / (1 + (m - 1) w)."""
+    at = {"first": 0, "last": m - 1, "inside": m // 3}[sink]
+    g, page = gen(40), 64
+    for f8 in (False, True):
+        pages = -(-m // page)
+        kc = torch.zeros(pages, hk, page, d, dtype=HF, device=DEV)
+        vc = (0.5 + torch.rand(pages, 1, page, d, generator=g, device=DEV)).to(HF)
+        vc = (vc.to(F8) if f8 else vc).expand(pages, hk, page, d).contiguous()
+        kc[at // page, :, at % page, 0] = 16.0
+        vc.view(torch.uint8 if f8 else torch.int16)[at // page, :, at % page] = 0
+        kc = kc.to(F8) if f8 else kc
+        one = dict(k_scale=torch.ones(hk, device=DEV), v_scale=torch.ones(hk, device=DEV)) if f8 else {}
+        q = torch.zeros(seqs * n, hq, d, dtype=HF, device=DEV)
+        q[..., 0] = 1.0
+        table = torch.arange(pages, dtype=torch.int32, device=DEV)[None].expand(seqs, pages)  # the same history
+        cu, lens = torch.arange(seqs + 1, dtype=torch.int32, device=DEV) * n, torch.full((seqs,), m, dtype=torch.int32, device=DEV)
+        v = vc[:, 0].reshape(-1, d)[:m].double()
+        for gap in (8.0, 14.0, 17.0, 20.0):
+            o, lse = ops.attn_paged_fwd(q, kc, vc, table, cu, lens, gap / 16, causal=False, **one)
+            w = math.exp(-gap)
+            ref, rl = w * v.sum(0) / (1 + (m - 1) * w), gap + math.log1p((m - 1) * w)
+            # check()'s bound, with probabilities held down to 2^-24 of fp16 at 2^10 for the largest: off by 2^-35 of it each
+            e32 = (d + 8) * R.F32U * gap + 8 * R.F32U * rl + (m / 4 + 128) * R.F32U
+            bound = (2 * R.U[HF] + 2 * e32) * ref * (1 + R.U[HF]) + 2.0 ** -35 * v.sum(0) + 2.0 ** -25
+            off = (o.double() - ref).abs() - bound
+            assert bool((off <= 0).all()), (f8, gap, float(((o.double() - ref).abs() / ref).max()))
+            assert float((lse.double() - rl).abs().max()) <= e32, (f8, gap)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("new,lens", [([1, 2], [700, 500]), ([200, 70], [900, 700]), ([300] * 60, [300 + 7 * i for i in range(60)])])
+def test_fp16_scores_that_rise_along_the_keys(new, lens, d):
+    """Every block's largest score exceeds all before it, by less and by more than what the running maximum tolerates."""
+    for hk, f8 in ((2, False), (8, False), (2, True)):
+        for slope in (0.002, 0.03, 0.3, 3.0):
+            s = batch(new, lens, 16, 2 * hk, hk, d, HF, f8, seed=41)
+            s["q"][..., 0] = 1.0
+            for b, m in enumerate(lens):
+                pl = torch.arange(m, device=DEV)
+                rise = (slope * pl / d ** -0.5).clamp(max=400.0 if f8 else 3e4)
+                if f8:
+                    s["kc"][s["table"][b].long()[pl // 16], :, pl % 16, 0] = (rise[:, None] / s["k_scale"]).clamp(max=448).to(F8)
+                else:
+                    s["kc"][s["table"][b].long()[pl // 16], :, pl % 16, 0] = rise[:, None].to(HF)
+            check(s, call(s, d ** -0.5), d ** -0.5, True, 0)
