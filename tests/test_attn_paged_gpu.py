@@ -1,11 +1,12 @@
 """hma_amd.ops.attn_paged_fwd on the GPU against softmax attention in 64 bits, and a run of kv_append + attn_paged as a rollout makes it."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import hma_amd.torch_ops  # noqa: F401
-from hma_amd import ops
+from hma_amd import _lib, ops
 from tests import rope_ref as R
 
 pytestmark = pytest.mark.gpu
@@ -434,3 +435,40 @@ def test_fp16_scores_that_rise_along_the_keys(new, lens, d):
                 else:
                     s["kc"][s["table"][b].long()[pl // 16], :, pl % 16, 0] = rise[:, None].to(HF)
             check(s, call(s, d ** -0.5), d ** -0.5, True, 0)
+
+
+def workspace(s, causal=True, window=0):
+    """Bytes that a call wants; none: its row tiles are not split along the keys."""
+    q, kc, n = s["q"], s["kc"], C.c_int64()
+    p = _lib.AttnPaged(tokens=q.shape[0], hq=q.shape[1], hk=kc.shape[1], d=q.shape[2], dtype=0 if q.dtype == BF else 1, seqs=len(s["new"]),
+                       table_w=s["table"].shape[1], pages=kc.shape[0], page=kc.shape[2], cache_e4m3=kc.dtype == F8, causal=causal, window=window, scale=1.0)
+    _lib.check(_lib.load().hma_attn_paged_ws(C.byref(p), C.byref(n)), "hma_attn_paged_ws")
+    return n.value
+
+
+UNSPLIT = {  # heads, key heads, new, lens, page, causal, window, tail
+    "one prompt": (140, 140, [1950], [1950], 32, True, 0, 0),
+    "a prompt behind a past": (160, 160, [1801, 1], [2500, 70], 16, True, 0, 3),
+    "many sequences, some idle": (17, 17, [0, 45, 80, 0, 45] * 24, [900, 45, 300, 0, 150] * 24, 16, True, 0, 5),
+    "odd pages": (34, 17, [33, 47, 0] * 40, [33, 130, 12] * 40, 7, True, 0, 0),
+    "window": (17, 17, [90, 45] * 60, [400, 45] * 60, 16, True, 30, 1),
+    "frames": (17, 17, [64] * 120, [64 * (1 + i % 5) for i in range(120)], 64, False, 0, 2),
+    "more new than cached": (17, 17, [70, 40] * 60, [50, 1] * 60, 48, True, 0, 0),
+}
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("name", list(UNSPLIT))
+def test_row_tiles_that_are_not_split(name, d):
+    hq, hk, new, lens, page, causal, window, tail = UNSPLIT[name]
+    for dtype, f8 in ((BF, False), (HF, False), (BF, True), (HF, True)):
+        s = batch(new, lens, page, hq, hk, d, dtype, f8, tail, seed=50 + d)
+        assert workspace(s, causal, window) == 0
+        o, lse = call(s, d ** -0.5, causal, window)
+        some = [0, hk // 2, hk - 1]  # key heads looked at, with the heads that share them
+        rows = [j * (hq // hk) + i for j in some for i in range(hq // hk)]
+        part = dict(s, q=s["q"][:, rows], kc=s["kc"].view(torch.uint8 if f8 else dtype)[:, some].view(s["kc"].dtype),
+                    vc=s["vc"].view(torch.uint8 if f8 else dtype)[:, some].view(s["vc"].dtype))
+        if f8:
+            part |= dict(k_scale=s["k_scale"][some], v_scale=s["v_scale"][some])
+        check(part, (o[:, rows], lse[:, rows]), d ** -0.5, causal, window)
