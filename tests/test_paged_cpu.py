@@ -3,6 +3,8 @@ frequencies."""
 import contextlib
 import ctypes as C
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -239,6 +241,25 @@ def test_rope_entries_refuse_their_own():
 
 def test_struct_sizes_match_the_header():
     assert C.sizeof(_lib.Rope) == 104 and C.sizeof(_lib.KvAppend) == 336 and C.sizeof(_lib.AttnPaged) == 232 and C.sizeof(_lib.QkRope) == 296
+
+
+def test_struct_layouts_are_the_header_s(tmp_path):
+    """Every field of the argument structures where the C header has it, asked of a C compiler."""
+    structs = {"hma_rope_t": _lib.Rope, "hma_qk_rope_t": _lib.QkRope, "hma_kv_append_t": _lib.KvAppend, "hma_attn_paged_t": _lib.AttnPaged}
+    lines = []
+    for name, cls in structs.items():
+        lines.append(f'printf("{name} - %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name} {f} %zu %zu\\n", offsetof({name}, {f}), sizeof((({name}*)0)->{f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"hma_hip.h\"\nint main(void) {\n" + "\n".join(lines) + "\nreturn 0;\n}\n")
+    subprocess.run(["gcc", "-I", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include"), str(src), "-o", str(exe)], check=True)
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, field, *n = line.split()
+        if field == "-":
+            assert C.sizeof(structs[name]) == int(n[0]), line
+        else:
+            f = getattr(structs[name], field)
+            assert [f.offset, f.size] == [int(x) for x in n], line
 
 
 # ------------------------------------------------------------------------------------------------ tracing, frequencies
