@@ -572,9 +572,11 @@ __global__ __launch_bounds__(TPB, 2) void attn_few_kernel(const Args a) {
 // register of lane offsets; a tile of keys is 16 such pieces at D = 128, four a wave.
 // Layout of a tile: piece = 64 / CPR rows (CPR = D / 8 chunks of 16 bytes each), pieces 16 bytes further apart than their size, chunk c of
 // row r at place c ^ turn(r) of its row.  A 16-byte read of 16 rows and a transposing read of 4 rows x 64 bytes then touch every bank once.
-// Two prompts of 5 to 8 K tokens, 32 heads of 128 on 8: 755 GFLOP in 780 us = 0.97 PFLOP/s, two thirds of what a large matrix product
-// reaches here (the matrix pipe is 44 % busy; the exponentials' instructions and the reads of LDS take the rest of a wave's turns).  Heads of
-// 32 have as many exponentials for a quarter of the products: 4 frames of 320 tokens over 5 to 20 K, 17 GFLOP in 51 us, the vector unit 70 % busy.
+// Two prompts of 5 to 8 K tokens, 32 heads of 128 on 8, 755 GFLOP: 763 to 790 us a launch back to back = 0.96 to 0.99 PFLOP/s, two thirds of what
+// a large matrix product reaches here (791 to 857 us apart from each other, under a trace).  Of a SIMD's cycles 49 % have a matrix instruction and 56 % a
+// vector one in work; a wave waits 32 % of its own.  Heads of 32 have as many exponentials for a quarter of the products: 4 frames of 320
+// tokens over 5 to 20 K, 17 GFLOP in 51 us, vector instructions in 69 % of the cycles (200 for 64 keys of 32 rows, 32 of them exponentials),
+// matrix instructions in 18 %, waves waiting 42 %.
 // Rejected, at the prompts: 64 rows a wave (one wave a SIMD) 862 us, 8 waves a workgroup the same, half tiles out of step slower.
 template <int D>
 struct Lay {

@@ -17,9 +17,10 @@
 // at position 10^6 is off by 0.03 rad.
 // Reductions: everything in 32 bits; each output is rounded once.
 // Measured (bf16): forward of 81920 tokens x 16 heads of 32, three axes, layer norm: 40 us = 4.2 TB/s of 168 MB; of 8191 x 40 heads of 128,
-// RMS norm: 34 us = 4.9 TB/s.  7 tokens x 40 heads of 128: 4.9 us, a launch and one trip to memory.  The cache form: 8 frames of 320 tokens x 32
+// RMS norm: 34 us = 4.9 TB/s.  fp32: 80 us = 4.2 TB/s and 71 us = 4.7 TB/s.
+// 7 tokens x 40 heads of 128: 4.9 us, a launch and one trip to memory.  The cache form: 8 frames of 320 tokens x 32
 // rows of 32: 12 us; 7.9 thousand tokens x 16 rows of 128 into e4m3: 21 us = 2.3 TB/s (what a wave does once, and four dependent loads in front
-// of its first store -- sequence, length, page, row -- for two tokens); 128 thousand such tokens: 250 us = 3.1 TB/s, into bf16 224 us =
+// of its first store -- sequence, length, page, row -- for two tokens); 128 thousand such tokens: 252 us = 3.1 TB/s, into bf16 224 us =
 // 4.7 TB/s; one token of 64 sequences x 48 rows of 128: 7.4 us.
 #include "hma_common.h"
 #include "../../include/hma_hip.h"
@@ -512,7 +513,8 @@ struct BwdArgs {
 // dx of every row; the sums for the weights per workgroup (a lane adds its 8 columns over all its rows in registers, the workgroup adds
 // its lanes in a fixed order), so no atomics and the same bits every time.  The sums of the tensor that a wave does not work on wait in
 // LDS: in registers they cost a wave of occupancy.  81920 tokens x 16 heads of 32, layer norm: 69 us = 3.7 TB/s of 252 MB; 8191 x 40 heads of
-// 128, RMS norm: 60 us = 4.2 TB/s; the second launch adds 768 partial sums in 4 us.
+// 128, RMS norm: 60 us = 4.2 TB/s; the second launch adds 768 partial sums in 4 us.  fp32, both launches:
+// 113 us = 4.5 TB/s and 107 us = 4.7 TB/s.
 template <typename T, int NORM, bool INTER>
 __global__ __launch_bounds__(TPB, Io<T>::SIZE == 2 ? 3 : 2) void rope_bwd_kernel(const BwdArgs g) {
   constexpr int U = 2, SZ = Io<T>::SIZE;

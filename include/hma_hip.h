@@ -601,7 +601,7 @@ enum { HMA_NORM_NONE = 0, HMA_NORM_RMS = 1, HMA_NORM_LAYER = 2 };
  * R turns pair i < rot / 2 -- values (2 i, 2 i + 1) if interleaved, else (i, i + rot / 2) -- by positions[axes[i]][token] * freqs[i]
  * radians and multiplies it by `amplitude`; values behind rot pass.  d % 8 == 0, d <= 256, rot even, 0 <= rot <= d.
  * freqs: double [rot / 2]; axes: int32 [rot / 2] or NULL (one axis); positions: [n_axes] rows pos_stride apart of int64 (pos_64) or
- * int32.  The angle is formed in 64 bits (exact to 1e-7 rad up to positions of 2^30).
+ * int32.  The angle is formed in 64 bits: off by at most 1e-7 rad + 3 * 2^-53 of it (4e-7 rad at 2^30 rad).
  * w / b of the norms ([d], NULL = 1 / 0; w_f32: fp32, else of the rows' type). */
 typedef struct {
   const double* freqs; const int32_t* axes; const void* positions; int64_t pos_stride;
