@@ -329,9 +329,10 @@ def _own(s):
         return ops.attn_paged_fwd(s["q"], s["kc"], s["vc"], s["table"], s["cu"], s["lens"], s["scale"], causal=s["causal"], window=s["window"],
                                   k_scale=s["ks"], v_scale=s["vs"])
     if s["op"] == "append":
-        q = ops.kv_append(s["k"], s["v"], s["kc"], s["vc"], s["table"], s["cu"], s["lens"], q=s["q"] if s["with_q"] else None, freqs=s["freqs"],
-                          positions=s["pos"], axes=s["axes"], interleaved=s["inter"], amplitude=s["amp"], norm=s["norm"], q_weight=s["qw"],
-                          q_bias=s["qb"], k_weight=s["kw"], k_bias=s["kb"], eps=s["eps"], k_scale=s["ks"], v_scale=s["vs"])
+        of_q = dict(q=s["q"], q_weight=s["qw"], q_bias=s["qb"]) if s["with_q"] else {}  # (its weights without it are refused)
+        q = ops.kv_append(s["k"], s["v"], s["kc"], s["vc"], s["table"], s["cu"], s["lens"], **of_q, freqs=s["freqs"], positions=s["pos"],
+                          axes=s["axes"], interleaved=s["inter"], amplitude=s["amp"], norm=s["norm"], k_weight=s["kw"], k_bias=s["kb"],
+                          eps=s["eps"], k_scale=s["ks"], v_scale=s["vs"])
         return [s["kc"], s["vc"]] + ([q] if s["with_q"] else [])
     if not s["grad"]:
         return ops.qk_rope_fwd(s["q"], s["k"], s["freqs"], s["pos"], axes=s["axes"], interleaved=s["inter"], amplitude=s["amp"], norm=s["norm"],
