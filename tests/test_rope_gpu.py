@@ -3,6 +3,7 @@ import itertools
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import hma_amd.torch_ops  # noqa: F401
 from hma_amd import ops
@@ -453,3 +454,20 @@ def test_append_rounds_the_quotient(dtype):
         want = (x.float() / s[:, None]).clamp(-448, 448).to(F8)
         off = got.view(torch.uint8) != want.view(torch.uint8)
         assert not off.any(), (int(off.sum()), s[off.any(0).any(-1)].tolist(), x[off][:4].tolist(), got[off][:4].float().tolist(), want[off][:4].float().tolist())
+
+
+def test_traced_graph_on_the_gpu():
+    """A graph traced with real tensors launches what the eager pass launches, forward and back, on inputs other than the trace's."""
+    def step(q, k, w, freqs, positions):
+        leaves = [t.detach().requires_grad_() for t in (q, k, w)]
+        y = torch.ops.hma.qk_rope(leaves[0], leaves[1], freqs, positions, None, True, 1.0, "rms", leaves[2], None, leaves[2], None, 1e-5)
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, leaves, [y[0].detach() * 2, y[1].detach()]))
+
+    a, b = (make(40, 6, 2, 64, 32, "rms", BF, seed=s) for s in (80, 81))
+    graph = make_fx(step)(a["q"], a["k"], a["q_weight"], a["freqs"], a["positions"])
+    called = [n.target for n in graph.graph.nodes if n.op == "call_function"]
+    assert called.count(torch.ops.hma.qk_rope.default) == 1 and called.count(torch.ops.hma.qk_rope_bwd.default) == 1
+    for s in (a, b):
+        args = (s["q"], s["k"], s["q_weight"], s["freqs"], s["positions"])
+        got, want = graph(*args), step(*args)
+        assert len(got) == len(want) == 5 and all(torch.equal(x, y) for x, y in zip(got, want))
